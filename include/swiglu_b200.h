@@ -267,6 +267,90 @@ int swiglu_b200_fused_matmul_swiglu_e4m3(const void* xq, const float* x_scale, c
 int swiglu_b200_matmul_e4m3(const void* aq, const float* a_scale, const void* bq, const float* b_scale, void* c,
                             int64_t M, int64_t N, int64_t K, int out_dtype, int group_size_m, void* stream);
 
+/* Residual RMS norm in front of the block. No counterpart in the reference,
+ * which starts at x. Over rows [rows, cols] of `dtype` (F32 or BF16) with a
+ * weight [cols] of `weight_dtype`:
+ *   s = x + residual, rounded to dtype and stored in s; with residual NULL the
+ *       stream is x itself and s (may be NULL) is not written
+ *   rstd [rows] = (mean of s^2 over the row + eps)^-1/2, f32
+ *   y = s * rstd * weight, in dtype
+ * eps is read on the host during the call (as BLAS scalars are).
+ * Statistics are f32. Any cols >= 1; pointers aligned to their element (16-byte
+ * alignment of every row takes the faster kernels). s may alias x or residual. */
+int swiglu_b200_rmsnorm_fwd(const void* x, const void* residual, const void* weight, void* y, void* s, float* rstd,
+                            int64_t rows, int64_t cols, const float* eps, int dtype, int weight_dtype, void* stream);
+
+/* The same with y as row-scaled e4m3, the operand of the e4m3 GEMMs below
+ * (swiglu_b200_quantize_rows_e4m3's convention): q = e4m3(y * 448 / amax),
+ * row_scale = amax / 448 (1 for an all-zero row; NaN where a row holds a NaN or
+ * an infinity), from the f32 y (no rounding to dtype in between). */
+int swiglu_b200_rmsnorm_fwd_e4m3(const void* x, const void* residual, const void* weight, void* q, float* row_scale,
+                                 void* s, float* rstd, int64_t rows, int64_t cols, const float* eps, int dtype,
+                                 int weight_dtype, void* stream);
+
+/* Floats of the workspace swiglu_b200_rmsnorm_bwd needs on a device with
+ * `num_sms` SMs. Host-only. */
+int swiglu_b200_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int num_sms, int64_t* floats);
+
+/* Gradient of the norm: from dy [rows, cols] (gradient of y), the stored s and
+ * rstd, and ds (gradient of s from its other uses, may be NULL),
+ *   dx = rstd * (dy * weight - s * rstd^2 * mean(dy * weight * s)) + ds
+ * (the gradient of x and of the residual alike, in dtype) and
+ *   dweight [cols] = sum over rows of dy * s * rstd (in weight_dtype).
+ * Sums are f32 in an order fixed by the sizes: results are run-to-run
+ * identical. workspace: 16-byte aligned device memory. */
+int swiglu_b200_rmsnorm_bwd(const void* dy, const void* s, const void* weight, const float* rstd, const void* ds,
+                            void* dx, void* dweight, float* workspace, int64_t workspace_floats, int64_t rows,
+                            int64_t cols, int dtype, int weight_dtype, void* stream);
+
+/* Global norm of a list of gradients and clipping by it (the step between a
+ * backward and its optimizer; the reference stops at the gradients). grads,
+ * outs, sizes (elements) and dtypes are host arrays of `count`; F32 and BF16
+ * tensors may be mixed, sizes may be 0, pointers need the alignment of their
+ * element only; max_norm is read on the host. workspace: device memory of
+ * swiglu_b200_grad_norm_workspace(count, SMs of the device) doubles. Sums are
+ * f64 above 64 values, in a fixed order.
+ *   grad_norm:          norm (device f32) = sqrt(sum of all squares)
+ *   clip_grad_norm:     and outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6));
+ *                       outs[i] == grads[i] scales in place (and leaves a tensor
+ *                       whose factor is 1 alone); a written tensor must not
+ *                       overlap any other of the call
+ *   clip_grads_by_norm: the scaling alone, by a norm already on the device
+ *                       (summed over the ranks of a sharded model, for instance). */
+int swiglu_b200_grad_norm_workspace(int64_t count, int num_sms, int64_t* doubles);
+int swiglu_b200_grad_norm(const void* const* grads, const int64_t* sizes, const int* dtypes, int64_t count,
+                          double* workspace, int64_t workspace_doubles, float* norm, void* stream);
+int swiglu_b200_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes,
+                               int64_t count, const double* max_norm, double* workspace, int64_t workspace_doubles,
+                               float* norm, void* stream);
+int swiglu_b200_clip_grads_by_norm(const void* const* grads, void* const* outs, const int64_t* sizes,
+                                   const int* dtypes, int64_t count, const float* norm, const double* max_norm,
+                                   void* stream);
+
+/* MXFP4 operand path (OCP Microscaling Formats v1.0): e2m1 codes, two to a
+ * byte (even column low), with one e8m0 scale per 32 columns. No counterpart in
+ * the reference. Block of 32: E = floor(log2 max|v|) - 2, codes e2m1(v * 2^-E)
+ * to nearest even, saturating at 6; scale byte E + 127 (at least 0; 255 = NaN
+ * where the block holds a NaN or an infinity). scale holds
+ * [ceil(rows / 128)][ceil(cols / 128)] tiles of 512 bytes; the byte of (row,
+ * block) is at (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4 of tile
+ * [row / 128][block / 4]; bytes beyond the matrix are 0.
+ *
+ * Quantises src [rows, cols] (F32 or BF16, cols % 32 == 0) into dst
+ * [rows, cols / 2] bytes and scale. 16-byte aligned pointers. */
+int swiglu_b200_quantize_mxfp4(const void* src, void* dst, void* scale, int64_t rows, int64_t cols, int dtype,
+                               void* stream);
+
+/* The values that codes and scales stand for, in dtype (exact). */
+int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, int64_t rows, int64_t cols, int dtype,
+                                 void* stream);
+
+/* C [M, N] = A . B^T for MXFP4 A [M, K] and B [N, K] with their scales, f32
+ * accumulation, C in out_dtype. K % 32 == 0, N % 8 == 0; the MXFP4 form of
+ * swiglu_b200_matmul_e4m3. */
+int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
+                             int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
+
 /* Whole forward of one MLP block: preact (saved for backward), h (caller's
  * transient workspace [M, H]) and y [M, Dout].
  * SwiGLUMemoryOptimizedFunction.forward (swiglu_recompute.py:59-66),

@@ -11,6 +11,7 @@
 #include <mutex>
 #include <string>
 
+#include "host.cuh"
 #include "simt_kernels.cuh"
 #include "tc_dw2.cuh"
 #include "tc_gemm2.cuh"
@@ -24,6 +25,7 @@ namespace {
 
 thread_local std::string t_last_error;
 
+}  // namespace
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -37,20 +39,13 @@ int fail(int code, const char* fmt, ...) {
 int cuda_fail(cudaError_t e, const char* what) {
   return fail(SWIGLU_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
+namespace {
 
-constexpr int kMaxDevices = 64;
 // Tile-order group (in 128-row tiles) for the GEMMs whose caller passes none:
 // 32 (16 pair rows) measured at config 2 against 16: GEMM1 1.618 -> 1.590 ms
 // with DRAM reads 1.87 -> 1.06 GB, y/dW1/dx within 0.2 %; walking every row
 // tile per column band (88) doubled the DRAM reads (3.65 GB).
 constexpr int kDefaultGroupM = 32;
-
-struct DeviceInfo {
-  std::atomic<bool> ready{false};
-  int sms = 0;
-  int major = 0;
-  uint32_t* status = nullptr;
-};
 
 std::mutex g_mu;
 DeviceInfo g_dev[kMaxDevices];
@@ -97,6 +92,7 @@ int resolve_device(int* out) {
   return SWIGLU_OK;
 }
 
+}  // namespace
 int current_device(DeviceInfo** out) {
   int dev = 0;
   cudaError_t e = cudaSuccess;
@@ -123,12 +119,10 @@ int current_device(DeviceInfo** out) {
   *out = &d;
   return SWIGLU_OK;
 }
+namespace {
 
 // ------------------------------------------------------------ tensor maps
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
+}  // namespace
 int get_encode_fn(EncodeTiledFn* out) {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -143,6 +137,7 @@ int get_encode_fn(EncodeTiledFn* out) {
   *out = fn;
   return SWIGLU_OK;
 }
+namespace {
 
 // 2-D bf16 map over a row-major [outer, inner] view with row pitch `ld`
 // elements; 128-byte swizzled boxes of {64, box_outer}.
@@ -168,6 +163,7 @@ int make_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, ui
 
 // Output map of a store GEMM: row-major [M, N] (pitch ld elements) in
 // {32 x 32} boxes, 64-byte swizzle for bf16 rows of 64 bytes, 128-byte for f32.
+}  // namespace
 int make_store_map(CUtensorMap* m, void* ptr, uint64_t N, uint64_t M, uint64_t ld, bool f32) {
   EncodeTiledFn fn;
   if (int rc = get_encode_fn(&fn)) return rc;
@@ -185,6 +181,7 @@ int make_store_map(CUtensorMap* m, void* ptr, uint64_t N, uint64_t M, uint64_t l
   if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "C: cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return SWIGLU_OK;
 }
+namespace {
 
 // 4-D bf16 map gathering several 64-column blocks of a row-major matrix in
 // one TMA operation: dims {64 columns, rows, blocks, groups} with byte
@@ -210,9 +207,8 @@ int make_map_gather4(CUtensorMap* m, const void* ptr, uint64_t rows, uint64_t ld
   return SWIGLU_OK;
 }
 
-// e4m3 operand map: row-major [rows, K] bytes, row pitch `ld` bytes; 128-byte
-// swizzled boxes of {128 elements of K, box_rows rows}.
-int make_map_e4m3(CUtensorMap* m, const void* ptr, uint64_t K, uint64_t rows, uint64_t ld, uint32_t box_rows,
+}  // namespace
+int make_map_bytes(CUtensorMap* m, const void* ptr, uint64_t K, uint64_t rows, uint64_t ld, uint32_t box_rows,
                   const char* what) {
   EncodeTiledFn fn;
   if (int rc = get_encode_fn(&fn)) return rc;
@@ -231,6 +227,7 @@ int make_map_e4m3(CUtensorMap* m, const void* ptr, uint64_t K, uint64_t rows, ui
   if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
   return SWIGLU_OK;
 }
+namespace {
 
 // Operand maps. K-major operand stored [rows][K]; MN-major stored [K][cols].
 int map_kmajor(CUtensorMap* m, const void* p, int64_t rows, int64_t K, int64_t ld, uint32_t box_rows,
@@ -253,92 +250,9 @@ std::atomic<int> g_gemm_path{0};
 // that kernels of other streams, e.g. NCCL collectives overlapped with the
 // GEMMs, find SMs to run on.
 std::atomic<int> g_sm_reserve{0};
-
-// Per-kernel launch state: dynamic shared memory opt-in done (bit per device)
-// and, for cluster kernels, how many CTA pairs fit at once on each device.
-struct KernelState {
-  std::atomic<uint64_t> ready{0};
-  int max_clusters[kMaxDevices] = {};
-};
-
-template <auto Kernel>
-KernelState& kernel_state() {
-  static KernelState s;  // one per kernel function
-  return s;
-}
-
-// Persistent single-CTA launch: one CTA per SM (at most one per tile).
-template <auto kern, class Params>
-int launch_single(const Params& p, int tiles, int threads, int smem, const DeviceInfo& d, cudaStream_t st,
-                  const char* what) {
-  KernelState& ks = kernel_state<kern>();
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!(ks.ready.load() & (1ull << dev))) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return cuda_fail(e, what);
-    ks.ready.fetch_or(1ull << dev);
-  }
-  int sms = d.sms - g_sm_reserve.load(std::memory_order_relaxed);
-  if (sms < 1) sms = 1;
-  const int grid = tiles < sms ? tiles : sms;
-  kern<<<grid, threads, smem, st>>>(p);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, what);
-}
-
-cudaLaunchConfig_t pair_launch_config(cudaLaunchAttribute* attr, int threads, int smem, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cfg;
-}
-
-// How many CTA pairs of `kern` fit on the current device at once (queried
-// once per device).
-template <auto kern>
-int pair_capacity(int threads, int smem, const DeviceInfo& d, int* out, const char* what) {
-  KernelState& ks = kernel_state<kern>();
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!(ks.ready.load() & (1ull << dev))) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return cuda_fail(e, what);
-    cudaLaunchAttribute attr[1];
-    cudaLaunchConfig_t cfg = pair_launch_config(attr, threads, smem, nullptr);
-    cfg.gridDim = dim3(2 * (d.sms / 2));
-    int n = 0;
-    e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
-    if (e != cudaSuccess) return cuda_fail(e, what);
-    if (n < 1) return fail(SWIGLU_ERR_CUDA, "%s: no CTA pair fits on device %d", what, dev);
-    ks.max_clusters[dev] = n;
-    ks.ready.fetch_or(1ull << dev);
-  }
-  const int keep = ks.max_clusters[dev] - (g_sm_reserve.load(std::memory_order_relaxed) + 1) / 2;
-  *out = keep < 1 ? 1 : keep;
-  return SWIGLU_OK;
-}
-
-// Persistent CTA-pair launch (clusters of 2): as many pairs as fit at once,
-// at most one per work unit.
-template <auto kern, class Params>
-int launch_pair(const Params& p, int units, int threads, int smem, const DeviceInfo& d, cudaStream_t st,
-                const char* what) {
-  int cap = 0;
-  if (int rc = pair_capacity<kern>(threads, smem, d, &cap, what)) return rc;
-  cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = pair_launch_config(attr, threads, smem, st);
-  cfg.gridDim = dim3(2 * (units < cap ? units : cap));
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, what);
-}
+}  // namespace
+int sm_reserve() { return g_sm_reserve.load(std::memory_order_relaxed); }
+namespace {
 
 // ------------------------------------------------------------ stream-K workspaces
 // A caller-owned device buffer per (device, stream), registered with
@@ -414,6 +328,7 @@ bool take_workspace(cudaStream_t st, uint8_t** ptr, size_t* bytes, uint32_t* epo
 // there are idle pairs for (at most kSkMaxSplit, each of at least
 // kSkMinBlocksPerPart blocks), if the stream has a workspace large enough.
 // `slabs` arrival counters are used per tail tile.
+}  // namespace
 void choose_stream_k(int tiles, int clusters, int num_kb, long long tile_floats, int slabs, cudaStream_t st,
                      float** partials, uint32_t** counters, int* tail_out, int* split_out, uint32_t* epoch_out) {
   *tail_out = 0;
@@ -442,6 +357,7 @@ void choose_stream_k(int tiles, int clusters, int num_kb, long long tile_floats,
   *split_out = split;
   *epoch_out = epoch;
 }
+namespace {
 
 template <class Cfg>
 int launch_tc(TcParams& p, const DeviceInfo& d, cudaStream_t st) {
@@ -563,12 +479,14 @@ int pointwise_grid(long long work, const DeviceInfo& d) {
   return g < 1 ? 1 : static_cast<int>(g);
 }
 
-bool fits_int(int64_t v) { return v >= 0 && v <= 0x7fffffffLL; }
 
+
+}  // namespace
 int check_dtype(int dtype) {
   if (dtype != SWIGLU_F32 && dtype != SWIGLU_BF16) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
   return SWIGLU_OK;
 }
+namespace {
 int check_layout(int layout, int64_t H) {
   if (layout != SWIGLU_LAYOUT_STD && layout != SWIGLU_LAYOUT_PACKED128)
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "unknown layout %d", layout);
@@ -576,6 +494,7 @@ int check_layout(int layout, int64_t H) {
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "packed layout needs H %% 128 == 0 (H=%lld)", (long long)H);
   return SWIGLU_OK;
 }
+}  // namespace
 int check_dims(const char* what, int64_t a, int64_t b, int64_t c) {
   if (!fits_int(a) || !fits_int(b) || !fits_int(c))
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: dimensions must be in [0, 2^31)", what);
@@ -585,6 +504,7 @@ int check_mult8(const char* what, int64_t v) {
   if (v % 8) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s=%lld must be a multiple of 8", what, (long long)v);
   return SWIGLU_OK;
 }
+namespace {
 
 // ---------------------------------------------------------------- ops
 int op_swiglu_fwd(const void* x, const void* w, void* preact, void* h, int64_t M, int64_t K, int64_t H, int dtype,
@@ -1077,8 +997,8 @@ int op_swiglu_fwd_e4m3(const void* xq, const float* x_scale, const void* wq, con
   DeviceInfo* d;
   if (int rc = current_device(&d)) return rc;
   TcParams p{};
-  if (int rc = make_map_e4m3(&p.tmA, xq, K, M, K, 128, "x (e4m3)")) return rc;
-  if (int rc = make_map_e4m3(&p.tmB, wq, K, 2 * H, K, 128, "W1 (e4m3)")) return rc;
+  if (int rc = make_map_bytes(&p.tmA, xq, K, M, K, 128, "x (e4m3)")) return rc;
+  if (int rc = make_map_bytes(&p.tmB, wq, K, 2 * H, K, 128, "W1 (e4m3)")) return rc;
   if (preact) {
     if (int rc = make_store_map(&p.tmC, preact, 2 * H, M, 2 * H, false)) return rc;
   }
@@ -1112,8 +1032,8 @@ int op_matmul_e4m3(const void* aq, const float* a_scale, const void* bq, const f
   DeviceInfo* d;
   if (int rc = current_device(&d)) return rc;
   TcParams p{};
-  if (int rc = make_map_e4m3(&p.tmA, aq, K, M, K, 128, "A (e4m3)")) return rc;
-  if (int rc = make_map_e4m3(&p.tmB, bq, K, N, K, 128, "B (e4m3)")) return rc;
+  if (int rc = make_map_bytes(&p.tmA, aq, K, M, K, 128, "A (e4m3)")) return rc;
+  if (int rc = make_map_bytes(&p.tmB, bq, K, N, K, 128, "B (e4m3)")) return rc;
   const bool f32 = out_dtype == SWIGLU_F32;
   if (int rc = make_store_map(&p.tmC, c, N, M, N, f32)) return rc;
   p.out0 = c;

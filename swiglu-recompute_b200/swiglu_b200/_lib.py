@@ -52,6 +52,17 @@ _SIGNATURES = {
     "swiglu_b200_quantize_rows_e4m3": [_p, _p, _p, _i64, _i64, _i, _p],
     "swiglu_b200_fused_matmul_swiglu_e4m3": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _i, _p],
     "swiglu_b200_matmul_e4m3": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _p],
+    "swiglu_b200_rmsnorm_fwd": [_p, _p, _p, _p, _p, _p, _i64, _i64, _p, _i, _i, _p],
+    "swiglu_b200_rmsnorm_fwd_e4m3": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p, _i, _i, _p],
+    "swiglu_b200_rmsnorm_bwd_workspace": [_i64, _i64, _i, ctypes.POINTER(_i64)],
+    "swiglu_b200_rmsnorm_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _p],
+    "swiglu_b200_grad_norm_workspace": [_i64, _i, ctypes.POINTER(_i64)],
+    "swiglu_b200_grad_norm": [_p, _p, _p, _i64, _p, _i64, _p, _p],
+    "swiglu_b200_clip_grad_norm": [_p, _p, _p, _p, _i64, _p, _p, _i64, _p, _p],
+    "swiglu_b200_clip_grads_by_norm": [_p, _p, _p, _p, _i64, _p, _p, _p],
+    "swiglu_b200_quantize_mxfp4": [_p, _p, _p, _i64, _i64, _i, _p],
+    "swiglu_b200_dequantize_mxfp4": [_p, _p, _p, _i64, _i64, _i, _p],
+    "swiglu_b200_matmul_mxfp4": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p],
     "swiglu_b200_mlp_forward":
         [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _p],
     "swiglu_b200_mlp_backward":

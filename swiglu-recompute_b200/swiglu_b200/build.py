@@ -56,7 +56,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     fd, tmp = tempfile.mkstemp(suffix=".so", dir=PKG_DIR)
     os.close(fd)
     cmd = [_nvcc(), "-std=c++17", "-O3", *ARCH_FLAGS, "-lineinfo",
-           "-Xcompiler", "-fPIC", "-shared", "-I", INCLUDE_DIR, "-I", CSRC_DIR,
+           "-Xcompiler", "-fPIC", "-shared", "-t", "0", "-I", INCLUDE_DIR, "-I", CSRC_DIR,
            "-o", tmp, *_sources()]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

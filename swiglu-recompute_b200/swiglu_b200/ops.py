@@ -9,6 +9,7 @@ native kernels on that device's current torch stream.
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -329,4 +330,231 @@ def matmul_e4m3(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_sca
     with torch.cuda.device(dev):
         _call(dev, "swiglu_b200_matmul_e4m3", _p(aq), _p(a_scale), _p(bq), _p(b_scale), _p(out), M, N, K,
               dtype_code(out_dtype), int(group_size_m), _stream(dev))
+    return out
+
+
+# ----------------------------------------------------------- helpers of the calls below
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """`name(*args, stream)` with `dev` current, on its current torch stream.
+    (Entering the device guard only where another device is current saves about
+    2 us a call, which single-token calls notice.)"""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch.cuda.current_device() == dev.index:
+        _call(dev, name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _call(dev, name, *args, stream)
+
+
+_sms: dict[int, int] = {}
+
+
+def _num_sms(dev: torch.device) -> int:
+    if dev.index not in _sms:
+        _sms[dev.index] = torch.cuda.get_device_properties(dev).multi_processor_count
+    return _sms[dev.index]
+
+
+# ------------------------------------------------------------ residual RMS norm
+def _check_norm(x: torch.Tensor, weight: torch.Tensor, *same: torch.Tensor | None) -> tuple[torch.device, int, int]:
+    dev = _check_cuda(x, weight, *same)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"the norm takes rows [M, D] with D >= 1, got {tuple(x.shape)}")
+    M, D = x.shape
+    if weight.shape != (D,):
+        raise ValueError(f"weight {tuple(weight.shape)} does not match rows of {D}")
+    for t in same:
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"shapes differ: {tuple(t.shape)} and {tuple(x.shape)}")
+    _same_dtype(x, *same)
+    return dev, M, D
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
+    """(y, s, rstd): the residual RMS norm of rows x [M, D] (bf16 or f32).
+    s = x + residual rounded to x's dtype (x itself without a residual),
+    rstd [M] = (mean s^2 + eps)^-1/2 in f32, y = s * rstd * weight in x's dtype.
+    weight [D] may be bf16 or f32."""
+    dev, M, D = _check_norm(x, weight, residual)
+    dt, wdt = dtype_code(x.dtype), dtype_code(weight.dtype)
+    y = torch.empty_like(x)
+    s = x if residual is None else torch.empty_like(x)
+    rstd = torch.empty((M,), device=dev, dtype=torch.float32)
+    _launch(dev, "swiglu_b200_rmsnorm_fwd", x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
+            s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(eps)), dt, wdt)
+    return y, s, rstd
+
+
+def rmsnorm_fwd_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+                     eps: float = 1e-6):
+    """(q, scale, s, rstd): rmsnorm_fwd with y as row-scaled e4m3 (q [M, D],
+    f32 scale [M], as quantize_rows_e4m3 gives them, but from the f32 y)."""
+    dev, M, D = _check_norm(x, weight, residual)
+    dt, wdt = dtype_code(x.dtype), dtype_code(weight.dtype)
+    q = torch.empty((M, D), device=dev, dtype=torch.float8_e4m3fn)
+    scale = torch.empty((M,), device=dev, dtype=torch.float32)
+    s = x if residual is None else torch.empty_like(x)
+    rstd = torch.empty((M,), device=dev, dtype=torch.float32)
+    _launch(dev, "swiglu_b200_rmsnorm_fwd_e4m3", x.data_ptr(), _ptr(residual), weight.data_ptr(), q.data_ptr(),
+            scale.data_ptr(), s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(eps)), dt, wdt)
+    return q, scale, s, rstd
+
+
+def rmsnorm_bwd(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                ds: torch.Tensor | None = None):
+    """(dx, dweight) of the norm: dx [M, D] is the gradient of x and of the
+    residual alike (ds, the gradient of s from its other uses, is added),
+    dweight [D] in weight's dtype. s and rstd as the forward returned them."""
+    dev, M, D = _check_norm(s, weight, dy, ds)
+    if rstd.device != dev or rstd.dtype != torch.float32 or rstd.shape != (M,) or not rstd.is_contiguous():
+        raise ValueError("rstd must be the forward's f32 [M] tensor")
+    dt, wdt = dtype_code(s.dtype), dtype_code(weight.dtype)
+    dx = torch.empty_like(s)
+    dweight = torch.empty_like(weight)
+    floats = ctypes.c_int64(0)
+    _lib.call("swiglu_b200_rmsnorm_bwd_workspace", M, D, _num_sms(dev), ctypes.byref(floats))
+    ws = torch.empty((floats.value,), device=dev, dtype=torch.float32)
+    _launch(dev, "swiglu_b200_rmsnorm_bwd", dy.data_ptr(), s.data_ptr(), weight.data_ptr(), rstd.data_ptr(),
+            _ptr(ds), dx.data_ptr(), dweight.data_ptr(), ws.data_ptr(), floats.value, M, D, dt, wdt)
+    return dx, dweight
+
+
+# --------------------------------------------------- gradient norm and clipping
+class _GradList:
+    """Host arrays of a list of gradients, checked."""
+
+    def __init__(self, tensors, out=None):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise ValueError("no gradients given")
+        dev = self.tensors[0].device
+        for t in self.tensors:
+            if t.device != dev or not t.is_cuda or not t.is_contiguous():
+                _check_cuda(self.tensors[0], t)  # raises with what is wrong
+        self.dev = dev
+        self.dtypes = array("i", [dtype_code(t.dtype) for t in self.tensors])
+        self.sizes = array("q", [t.numel() for t in self.tensors])
+        self.grads = array("Q", [t.data_ptr() for t in self.tensors])
+        self.outs = self.grads
+        self.out = None
+        if out is not None:
+            self.out = list(out)
+            if len(self.out) != len(self.tensors):
+                raise ValueError(f"{len(self.out)} outputs for {len(self.tensors)} gradients")
+            for t, o in zip(self.tensors, self.out):
+                if o.shape != t.shape or o.dtype != t.dtype:
+                    raise ValueError("an output differs from its gradient in shape or dtype")
+                _check_cuda(t, o)
+            self.outs = array("Q", [o.data_ptr() for o in self.out])
+
+    def args(self, with_outs: bool):
+        a = [self.grads.buffer_info()[0]]
+        if with_outs:
+            a.append(self.outs.buffer_info()[0])
+        return (*a, self.sizes.buffer_info()[0], self.dtypes.buffer_info()[0], len(self.tensors))
+
+    def workspace(self) -> torch.Tensor:
+        n = ctypes.c_int64(0)
+        _lib.call("swiglu_b200_grad_norm_workspace", len(self.tensors), _num_sms(self.dev), ctypes.byref(n))
+        return torch.empty((n.value,), device=self.dev, dtype=torch.float64)
+
+    def written(self) -> None:
+        torch.autograd.graph.increment_version(self.tensors if self.out is None else self.out)
+
+
+def grad_norm(tensors) -> torch.Tensor:
+    """The 2-norm (f32, a 0-dim tensor on their device) of all the values of a
+    list of contiguous bf16 / f32 tensors on one device."""
+    g = _GradList(tensors)
+    norm = torch.empty((), device=g.dev, dtype=torch.float32)
+    ws = g.workspace()
+    _launch(g.dev, "swiglu_b200_grad_norm", *g.args(False), ws.data_ptr(), ws.numel(), norm.data_ptr())
+    return norm
+
+
+def clip_grad_norm_(tensors, max_norm: float, *, out=None) -> torch.Tensor:
+    """Scales the gradients by min(1, max_norm / (norm + 1e-6)), norm being
+    grad_norm(tensors), and returns the norm (before clipping, on the device:
+    nothing here waits for it). In place, or into the tensors `out`. A tensor
+    that is written may not share memory with another one of the call."""
+    g = _GradList(tensors, out)
+    norm = torch.empty((), device=g.dev, dtype=torch.float32)
+    ws = g.workspace()
+    _launch(g.dev, "swiglu_b200_clip_grad_norm", *g.args(True), ctypes.byref(ctypes.c_double(max_norm)), ws.data_ptr(), ws.numel(),
+            norm.data_ptr())
+    g.written()
+    return norm
+
+
+def clip_grads_by_norm_(tensors, norm: torch.Tensor, max_norm: float, *, out=None) -> None:
+    """clip_grad_norm_ with a norm that is already known: an f32 tensor of one
+    value on the gradients' device (reduced over ranks, for instance)."""
+    g = _GradList(tensors, out)
+    if norm.device != g.dev or norm.dtype != torch.float32 or norm.numel() != 1:
+        raise ValueError("norm must be one f32 value on the gradients' device")
+    _launch(g.dev, "swiglu_b200_clip_grads_by_norm", *g.args(True), norm.data_ptr(),
+            ctypes.byref(ctypes.c_double(max_norm)))
+    g.written()
+
+
+# ------------------------------------------------------------------- MXFP4 path
+def mxfp4_scale_shape(rows: int, cols: int) -> tuple[int, int, int, int, int]:
+    """Shape of the scale tensor of a [rows, cols] MXFP4 matrix: tiles of 128
+    rows by 4 blocks; the byte of (row, block) is element [row // 128,
+    block // 4, row % 32, (row % 128) // 32, block % 4]."""
+    return (-(-rows // 128), -(-cols // 128), 32, 4, 4)
+
+
+def _check_mx(q: torch.Tensor, scale: torch.Tensor) -> tuple[int, int]:
+    if q.dtype != torch.uint8 or scale.dtype != torch.uint8 or q.dim() != 2:
+        raise TypeError("an MXFP4 matrix is a uint8 [R, K / 2] tensor of codes and a uint8 tensor of scales")
+    R, K = q.shape[0], 2 * q.shape[1]
+    if tuple(scale.shape) != mxfp4_scale_shape(R, K):
+        raise ValueError(f"scales {tuple(scale.shape)} do not fit a [{R}, {K}] matrix: {mxfp4_scale_shape(R, K)}")
+    return R, K
+
+
+def quantize_mxfp4(t: torch.Tensor):
+    """(q, scale): MXFP4 copy of a bf16 or f32 [R, K] matrix, K % 32 == 0: q
+    uint8 [R, K / 2] (two e2m1 codes a byte, the even column low) and the e8m0
+    scale bytes in the product's tiles (mxfp4_scale_shape)."""
+    dev = _check_cuda(t)
+    if t.dim() != 2:
+        raise ValueError(f"quantize_mxfp4 takes a matrix, got {tuple(t.shape)}")
+    R, K = t.shape
+    if K % 32:
+        raise ValueError(f"{K} columns are not a multiple of 32")
+    dt = dtype_code(t.dtype)
+    q = torch.empty((R, K // 2), device=dev, dtype=torch.uint8)
+    scale = torch.empty(mxfp4_scale_shape(R, K), device=dev, dtype=torch.uint8)
+    _launch(dev, "swiglu_b200_quantize_mxfp4", t.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, dt)
+    return q, scale
+
+
+def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The [R, K] values of an MXFP4 matrix, in bf16 or f32 (exact)."""
+    dev = _check_cuda(q, scale)
+    R, K = _check_mx(q, scale)
+    out = torch.empty((R, K), device=dev, dtype=dtype)
+    _launch(dev, "swiglu_b200_dequantize_mxfp4", q.data_ptr(), scale.data_ptr(), out.data_ptr(), R, K,
+            dtype_code(dtype))
+    return out
+
+
+def matmul_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_scale: torch.Tensor, *,
+                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """C [M, N] = A . B^T for MXFP4 A [M, K] and B [N, K] with their scales;
+    N % 8 == 0."""
+    dev = _check_cuda(aq, a_scale, bq, b_scale)
+    M, K = _check_mx(aq, a_scale)
+    N, K2 = _check_mx(bq, b_scale)
+    if K != K2:
+        raise ValueError(f"inner dimensions differ: {K} vs {K2}")
+    out = torch.empty((M, N), device=dev, dtype=out_dtype)
+    _launch(dev, "swiglu_b200_matmul_mxfp4", aq.data_ptr(), a_scale.data_ptr(), bq.data_ptr(), b_scale.data_ptr(),
+            out.data_ptr(), M, N, K, dtype_code(out_dtype))
     return out
