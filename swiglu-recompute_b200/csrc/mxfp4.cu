@@ -18,14 +18,14 @@
 #include <cuda_fp4.h>
 
 #include "host.cuh"
-#include "ptx.cuh"
+#include "tc_mxfp4.cuh"
 
 namespace swiglu {
 namespace {
 
 constexpr int kBlock = 32;          // columns that share a scale
 constexpr int kTileRows = 128;
-constexpr int kTileBytes = 512;
+constexpr int kTileBytes = kMxTileBytes;
 constexpr int kQuantCols = 256;     // columns of one CTA: a warp covers a row of them, 8 a thread
 constexpr int kQuantThreads = 256;
 
@@ -170,62 +170,6 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_mxfp4_kernel(const u
   }
 }
 
-// C = A . B^T from the decoded values, f32 accumulation: 64 x 64 outputs a
-// CTA, one block of 32 along K at a time.
-__device__ __forceinline__ void decode_rows(const uint8_t* q, const uint8_t* scale, long long rows, long long r0, int K,
-                                            int tiles_k, int kb, float (*to)[kBlock + 1]) {
-  // 64 rows x 16 bytes: a thread decodes 4 bytes of one row.
-  const int rr = threadIdx.x >> 2, part = threadIdx.x & 3;
-  const long long r = r0 + rr;
-  uint32_t codes = 0;
-  float s = 0.0f;
-  if (r < rows) {
-    codes = *reinterpret_cast<const uint32_t*>(q + r * (K / 2) + kb * 16 + part * 4);
-    s = scale_value(scale[((r / kTileRows) * tiles_k + kb / 4) * kTileBytes + (r % 32) * 16 + (r % kTileRows) / 32 * 4 +
-                          kb % 4]);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 v = e2m1x2_value((codes >> (8 * e)) & 0xffu);
-    to[rr][part * 8 + 2 * e] = v.x * s;
-    to[rr][part * 8 + 2 * e + 1] = v.y * s;
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) matmul_mxfp4_kernel(const uint8_t* aq, const uint8_t* as, const uint8_t* bq,
-                                                           const uint8_t* bs, T* c, int M, int N, int K, int tiles_k) {
-  __shared__ float a[64][kBlock + 1], b[64][kBlock + 1];
-  const long long m0 = blockIdx.y * 64ll, n0 = blockIdx.x * 64ll;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int kb = 0; kb < K / kBlock; ++kb) {
-    __syncthreads();
-    decode_rows(aq, as, M, m0, K, tiles_k, kb, a);
-    decode_rows(bq, bs, N, n0, K, tiles_k, kb, b);
-    __syncthreads();
-#pragma unroll 8
-    for (int k = 0; k < kBlock; ++k) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += a[ty + 16 * i][k] * b[tx + 16 * j][k];
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N) {
-        if constexpr (sizeof(T) == 4) c[m * N + n] = acc[i][j];
-        else c[m * N + n] = __float2bfloat16_rn(acc[i][j]);
-      }
-    }
-  }
-}
-
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int check_mx(const char* what, int64_t rows, int64_t cols) {
@@ -287,32 +231,160 @@ int op_dequantize(const void* q, const void* scale, void* dst, int64_t rows, int
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "dequantize_mxfp4 launch");
 }
 
-int op_matmul(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c, int64_t M, int64_t N,
-              int64_t K, int out_dtype, cudaStream_t st) {
+// Scale tiles as rows of 32-bit cells, one row per 128 rows of the matrix; a
+// box is the two tiles of a stage.
+int make_map_scales(CUtensorMap* m, const void* ptr, int64_t rows, int64_t K, const char* what) {
+  EncodeTiledFn fn;
+  if (int rc = get_encode_fn(&fn)) return rc;
+  const cuuint64_t tiles_k = static_cast<cuuint64_t>((K + 127) / 128);
+  const cuuint64_t dims[2] = {tiles_k * (kMxTileBytes / 4), static_cast<cuuint64_t>((rows + 127) / 128)};
+  const cuuint64_t strides[1] = {tiles_k * kMxTileBytes};
+  const cuuint32_t box[2] = {kMxScaleBytes / 4, 1};
+  const cuuint32_t es[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(ptr), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
+  return SWIGLU_OK;
+}
+
+// How a product runs. few: the swapped kernel, `parts` CTAs of a cluster along
+// K per tile of 128 weight rows. Otherwise pair tiles, the last `tail` of them
+// split into `split` ranges of K, with `bytes` of workspace (arrival counters,
+// then the parts).
+struct MxPlan {
+  bool few;
+  int parts;
+  int tiles_m, tiles_n, tail, split;
+  size_t bytes;
+};
+constexpr int kFewRows = 128;
+constexpr size_t kMxCounterBytes = 4096;
+
+MxPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
+  MxPlan p{};
+  const int num_kb = static_cast<int>((K + kMxStageK - 1) / kMxStageK);
+  p.split = p.parts = 1;
+  if (M <= kFewRows) {
+    p.few = true;
+    // Clusters as long as all CTAs fit at once, two to an SM.
+    const int64_t tiles = (N + 127) / 128;
+    while (p.parts < 8 && 2 * p.parts * tiles <= 2 * sms && 2 * p.parts <= num_kb) p.parts *= 2;
+    return p;
+  }
+  p.tiles_m = static_cast<int>((M + 255) / 256);
+  p.tiles_n = static_cast<int>((N + 255) / 256);
+  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n, pairs = sms / 2 > 0 ? sms / 2 : 1;
+  const int64_t tail = tiles % pairs, rounds = (tiles + pairs - 1) / pairs;
+  // As the 2-SM kernels: only where a split saves 5 % of the pairs' rounds.
+  if (tail == 0 || (pairs - tail) * 20 < pairs * rounds) return p;
+  int64_t split = pairs / tail;
+  if (split > 16) split = 16;
+  if (split > num_kb / 4) split = num_kb / 4;
+  if (split < 2) return p;
+  p.tail = static_cast<int>(tail);
+  p.split = static_cast<int>(split);
+  p.bytes = kMxCounterBytes + static_cast<size_t>(tail * split) * 256 * 256 * 4;
+  return p;
+}
+
+int usable_sms(const DeviceInfo& d) {
+  const int sms = d.sms - sm_reserve();
+  return sms < 2 ? 2 : sms;
+}
+
+template <int NT, bool F32>
+int launch_few(const MxFewParams& p, const MxPlan& plan, cudaStream_t st) {
+  using Cfg = MxFewCfg<NT, F32>;
+  constexpr auto kern = mx_gemm_few_kernel<Cfg>;
+  KernelState& ks = kernel_state<kern>();
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ks.ready.load() & (1ull << dev))) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
+    if (e != cudaSuccess) return cuda_fail(e, "matmul_mxfp4 launch");
+    ks.ready.fetch_or(1ull << dev);
+  }
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = pair_launch_config(attr, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, st);
+  attr[0].val.clusterDim.x = plan.parts;
+  cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * plan.parts));
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "matmul_mxfp4 launch");
+}
+
+template <bool F32>
+int run_few(MxFewParams& p, const MxPlan& plan, cudaStream_t st) {
+  if (p.M <= 16) return launch_few<16, F32>(p, plan, st);
+  if (p.M <= 32) return launch_few<32, F32>(p, plan, st);
+  if (p.M <= 64) return launch_few<64, F32>(p, plan, st);
+  return launch_few<128, F32>(p, plan, st);
+}
+
+template <bool F32>
+int run_pair(MxParams& p, const DeviceInfo& d, cudaStream_t st) {
+  using Cfg = MxCfg<F32>;
+  return launch_pair<mx_gemm_pair_kernel<Cfg>>(p, p.tiles_m * p.tiles_n + p.sk_tail * (p.sk_split - 1),
+                                               Cfg::NUM_THREADS, Cfg::SMEM_BYTES, d, st, "matmul_mxfp4 launch");
+}
+
+int check_matmul(int64_t M, int64_t N, int64_t K) {
   if (int rc = check_mx("matmul_mxfp4", M, K)) return rc;
   if (int rc = check_mx("matmul_mxfp4", N, K)) return rc;
-  if (int rc = check_dtype(out_dtype)) return rc;
   if (K <= 0) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "K must be positive");
   if (int rc = check_mult8("N", N)) return rc;
+  if (((M + 255) / 256) * ((N + 255) / 256) > 0x7fffffff)
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "matmul_mxfp4: M=%lld, N=%lld make too many tiles", (long long)M,
+                (long long)N);
+  return SWIGLU_OK;
+}
+
+int op_matmul(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c, int64_t M, int64_t N,
+              int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+  if (int rc = check_matmul(M, N, K)) return rc;
+  if (int rc = check_dtype(out_dtype)) return rc;
   if (M == 0 || N == 0) return SWIGLU_OK;
   if (!aq || !a_scale || !bq || !b_scale || !c) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
-  if (!aligned16(aq) || !aligned16(a_scale) || !aligned16(bq) || !aligned16(b_scale) || !aligned16(c))
+  if (!aligned16(aq) || !aligned16(a_scale) || !aligned16(bq) || !aligned16(b_scale) || !aligned16(c) ||
+      !aligned16(workspace))
     return fail(SWIGLU_ERR_MISALIGNED, "matmul_mxfp4: pointers must be 16-byte aligned");
   DeviceInfo* d;
   if (int rc = current_device(&d)) return rc;
-  const dim3 grid(static_cast<unsigned>((N + 63) / 64), static_cast<unsigned>((M + 63) / 64));
-  if (grid.y > 65535) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "matmul_mxfp4: M=%lld is too large", (long long)M);
-  const int tiles_k = static_cast<int>((K + 127) / 128);
-  const auto *a = static_cast<const uint8_t*>(aq), *as = static_cast<const uint8_t*>(a_scale);
-  const auto *b = static_cast<const uint8_t*>(bq), *bs = static_cast<const uint8_t*>(b_scale);
-  if (out_dtype == SWIGLU_F32)
-    matmul_mxfp4_kernel<float><<<grid, 256, 0, st>>>(a, as, b, bs, static_cast<float*>(c), (int)M, (int)N, (int)K,
-                                                     tiles_k);
-  else
-    matmul_mxfp4_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, as, b, bs, static_cast<__nv_bfloat16*>(c), (int)M,
-                                                             (int)N, (int)K, tiles_k);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "matmul_mxfp4 launch");
+  const bool f32 = out_dtype == SWIGLU_F32;
+  const MxPlan plan = plan_matmul(M, N, K, usable_sms(*d));
+  if (plan.few) {
+    MxFewParams p{};
+    const uint32_t nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    if (int rc = make_map_bytes(&p.tmW, bq, K / 2, N, K / 2, 128, "B (MXFP4)")) return rc;
+    if (int rc = make_map_bytes(&p.tmX, aq, K / 2, M, K / 2, nt, "A (MXFP4)")) return rc;
+    if (int rc = make_map_scales(&p.tmWs, b_scale, N, K, "B scales")) return rc;
+    if (int rc = make_map_scales(&p.tmXs, a_scale, M, K, "A scales")) return rc;
+    p.out = c;
+    p.M = (int)M, p.N = (int)N, p.K = (int)K;
+    p.status = d->status;
+    return f32 ? run_few<true>(p, plan, st) : run_few<false>(p, plan, st);
+  }
+  if (static_cast<int64_t>(plan.bytes) > workspace_bytes || (plan.bytes && !workspace))
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "matmul_mxfp4: workspace of %lld bytes, %lld needed",
+                (long long)workspace_bytes, (long long)plan.bytes);
+  MxParams p{};
+  if (int rc = make_map_bytes(&p.tmA, aq, K / 2, M, K / 2, 128, "A (MXFP4)")) return rc;
+  if (int rc = make_map_bytes(&p.tmB, bq, K / 2, N, K / 2, 128, "B (MXFP4)")) return rc;
+  if (int rc = make_map_scales(&p.tmAs, a_scale, M, K, "A scales")) return rc;
+  if (int rc = make_map_scales(&p.tmBs, b_scale, N, K, "B scales")) return rc;
+  if (int rc = make_store_map(&p.tmC, c, N, M, N, f32)) return rc;
+  p.M = (int)M, p.N = (int)N, p.K = (int)K;
+  p.tiles_m = plan.tiles_m, p.tiles_n = plan.tiles_n;
+  p.group_m = 16;
+  p.status = d->status;
+  p.sk_tail = plan.tail, p.sk_split = plan.split;
+  if (plan.bytes) {
+    p.sk_counters = static_cast<uint32_t*>(workspace);
+    p.sk_partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kMxCounterBytes);
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, kMxCounterBytes, st);
+    if (e != cudaSuccess) return cuda_fail(e, "matmul_mxfp4 workspace");
+  }
+  return f32 ? run_pair<true>(p, *d, st) : run_pair<false>(p, *d, st);
 }
 
 }  // namespace
@@ -332,9 +404,20 @@ int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, in
   return op_dequantize(q, scale, dst, rows, cols, dtype, static_cast<cudaStream_t>(stream));
 }
 
+int swiglu_b200_matmul_mxfp4_workspace(int64_t M, int64_t N, int64_t K, int num_sms, int64_t* bytes) {
+  if (int rc = check_matmul(M, N, K)) return rc;
+  if (!bytes) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
+  if (num_sms < 1) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "num_sms must be positive");
+  const int sms = num_sms - sm_reserve();
+  *bytes = M && N ? static_cast<int64_t>(plan_matmul(M, N, K, sms < 2 ? 2 : sms).bytes) : 0;
+  return SWIGLU_OK;
+}
+
 int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
-                             int64_t M, int64_t N, int64_t K, int out_dtype, void* stream) {
-  return op_matmul(aq, a_scale, bq, b_scale, c, M, N, K, out_dtype, static_cast<cudaStream_t>(stream));
+                             int64_t M, int64_t N, int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  return op_matmul(aq, a_scale, bq, b_scale, c, M, N, K, out_dtype, workspace, workspace_bytes,
+                   static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

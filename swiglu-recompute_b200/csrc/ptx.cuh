@@ -188,6 +188,16 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
       : "r"(taddr)
       : "memory");
 }
+// The same for 16 columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Warp-wide store of 32 consecutive 32-bit TMEM columns, one lane per row
@@ -312,6 +322,42 @@ __device__ __forceinline__ void umma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc
       : "memory");
 }
 
+// MXFP4 MMAs (kind::mxf4, packed e2m1 operands, one e8m0 scale per 32 of K,
+// f32 accumulation): K = 64 per instruction, 32 bytes of each operand row. The
+// scales are read from TMEM columns `sfa` / `sfb`, from byte pair 0-1 or 2-3 of
+// each 32-bit cell as the instruction descriptor says.
+__device__ __forceinline__ void umma_mxf4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_mxf4_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                  uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+// Copies a 512-byte scale tile (32 rows of 16 bytes) from shared memory to
+// four TMEM columns, repeated over the four 32-lane quarters. Ordered before
+// the MMAs that the same thread issues after it. The pair form copies in each
+// CTA from its own shared memory.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // Arrive once on the mbarrier at `bar_cluster_addr` (this CTA's or the
 // peer's) when the pair MMAs issued so far by this thread complete.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
@@ -334,6 +380,17 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t saddr, uint32_
   return d;
 }
 
+// The same without a swizzle, for the scale tiles: 8-row groups of 16-byte rows
+// (128 contiguous bytes) every 128 bytes.
+__device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= 1ull << 46;
+  return d;
+}
+
 // Instruction descriptor for kind::f16 with f32 accumulation.
 // a_fmt/b_fmt: 0 = f16, 1 = bf16. Majors: 0 = K-major, 1 = MN-major.
 __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, int a_fmt, int b_fmt, int a_mn, int b_mn) {
@@ -349,6 +406,19 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, int a_fmt, i
 // Instruction descriptor for kind::f8f6f4 with e4m3 A and B (format code 0)
 // and f32 accumulation; both operands K-major.
 __host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) { return make_idesc_f16(M, N, 0, 0, 0, 0); }
+
+// Instruction descriptor for kind::mxf4: e2m1 operands (format code 1), e8m0
+// scales (bit 23), both K-major; `sf_id` (0 or 2) picks the byte pair of the
+// scale cells that holds this K = 64 step's two blocks.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int M, int N, int sf_id) {
+  return (static_cast<uint32_t>(sf_id) << 4)        // B scale bytes
+         | (1u << 7)                                // A format
+         | (1u << 10)                               // B format
+         | (static_cast<uint32_t>(N >> 3) << 17)    // N / 8
+         | (1u << 23)                               // e8m0 scales
+         | (static_cast<uint32_t>(M >> 7) << 27)    // M / 128
+         | (static_cast<uint32_t>(sf_id) << 29);    // A scale bytes
+}
 
 // ------------------------------------------------------------- numerics
 __device__ __forceinline__ float bf16_round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }

@@ -154,7 +154,7 @@ __device__ __forceinline__ bool sk_arrive_last(uint32_t* ctr, uint32_t epoch, in
 // `part_stride` floats apart, added in part order so the result does not
 // depend on which part finished last) in TMEM in place of its own part, and
 // the ordinary epilogue can run.
-__device__ __noinline__ bool sk_publish_and_fix(uint32_t t_row, int ncols, float* mine, const float* fix,
+static __device__ __noinline__ bool sk_publish_and_fix(uint32_t t_row, int ncols, float* mine, const float* fix,
                                                 long long part_stride, int parts, uint32_t* counter, uint32_t epoch) {
 #pragma unroll 1
   for (int c = 0; c < ncols; c += 32) {

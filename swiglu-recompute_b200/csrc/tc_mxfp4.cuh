@@ -1,0 +1,512 @@
+// MXFP4 products on the block-scaled tensor-core kind: C [M, N] = A . B^T for
+// A [M, K], B [N, K] in e2m1 codes with e8m0 scales (mxfp4.cu has the format).
+//
+// Per k-block of 256 elements a stage holds 128 bytes of each operand row
+// (128-byte swizzle, as the 8- and 16-bit kernels) and the scale tiles of the
+// same rows: two tiles of 512 bytes per 128 rows, copied by the MMA thread to
+// TMEM (tcgen05.cp) right before the four MMAs (K = 64 each) that use them.
+// Scale columns are double-buffered: the copy for k-block i waits for the MMAs
+// of k-block i - 2, so it runs under those of i - 1.
+//
+// Out-of-range rows, columns of K and scale tiles are filled with zeros by TMA:
+// a zero code times 2^-127 is zero, so no tail needs a case of its own.
+#pragma once
+
+#include "tc_gemm.cuh"
+
+namespace swiglu {
+
+constexpr int kMxStageK = 256;           // elements of K per stage (128 bytes)
+constexpr int kMxTileBytes = 512;        // one scale tile: 128 rows x 128 elements of K
+constexpr int kMxScaleBytes = 2 * kMxTileBytes;  // of 128 rows per stage
+
+// ------------------------------------------------------------ CTA pair, 256 x 256
+struct MxParams {
+  CUtensorMap tmA, tmB;    // codes, {128 bytes, 128 rows}
+  CUtensorMap tmAs, tmBs;  // scale tiles as 32-bit cells, {256, 1}: both tiles of a stage
+  CUtensorMap tmC;         // output, {32 x 32} boxes
+  int M, N, K;
+  int tiles_m, tiles_n, group_m;
+  uint32_t* status;
+  // Split of the last, partial round of tiles along K (see TcParams).
+  float* sk_partials;
+  uint32_t* sk_counters;
+  int sk_tail, sk_split;
+};
+
+// TMEM: two 256-column accumulators that share 64 columns (0..255 and
+// 192..447) leave 64 columns for the scales. The epilogue reads the shared
+// columns first and frees them, then the next tile's MMAs may start: with two
+// whole accumulators TMEM would be full.
+template <bool OUT_F32_>
+struct MxCfg {
+  static constexpr bool OUT_F32 = OUT_F32_;
+  static constexpr int STAGES = 5;
+  static constexpr int OPERAND_BYTES = 128 * 128;  // 128 rows
+  static constexpr int SFA_OFFSET = 2 * OPERAND_BYTES;
+  static constexpr int SFB_OFFSET = SFA_OFFSET + kMxScaleBytes;
+  static constexpr int STAGE_BYTES = SFB_OFFSET + 2 * kMxScaleBytes;
+  static constexpr int ACC_STEP = 192;  // accumulator 1 starts here
+  static constexpr int SF_COL = 448;    // scale buffers: 448 and 480, 24 columns each
+  static constexpr int NUM_THREADS = 192;
+  static constexpr int BAR_BYTES = 8 * (2 * STAGES + 4) + 16;
+  static constexpr int EPI_OFFSET = STAGES * STAGE_BYTES + ((BAR_BYTES + 1023) / 1024) * 1024;
+  static constexpr int SMEM_BYTES = 1024 + EPI_OFFSET + 4 * StoreStage<OUT_F32>::kWarpBytes;
+  static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+};
+
+// One {32 x 32} box of accumulator values to C through a swizzled staging
+// buffer (StoreStage describes it).
+template <bool OUT_F32>
+__device__ __forceinline__ void mx_store_chunk(const CUtensorMap* map, const uint32_t (&r)[32], uint8_t* buf, int col,
+                                               int row0) {
+  using S = StoreStage<OUT_F32>;
+  const uint32_t lane = threadIdx.x & 31u;
+  if (lane == 0) bulk_wait_read<1>();  // the store issued from this buffer two boxes ago has read it
+  __syncwarp();
+  uint8_t* row_base = buf + lane * S::kRowBytes;
+#pragma unroll
+  for (int k = 0; k < S::kRowBytes / 16; ++k) {
+    uint4 v;
+    if constexpr (OUT_F32) {
+      v = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+    } else {
+      v = make_uint4(pack_bf16x2(__uint_as_float(r[8 * k]), __uint_as_float(r[8 * k + 1])),
+                     pack_bf16x2(__uint_as_float(r[8 * k + 2]), __uint_as_float(r[8 * k + 3])),
+                     pack_bf16x2(__uint_as_float(r[8 * k + 4]), __uint_as_float(r[8 * k + 5])),
+                     pack_bf16x2(__uint_as_float(r[8 * k + 6]), __uint_as_float(r[8 * k + 7])));
+    }
+    const int kk = OUT_F32 ? (k ^ static_cast<int>(lane & 7u)) : (k ^ static_cast<int>((lane >> 1) & 3u));
+    *reinterpret_cast<uint4*>(row_base + 16 * kk) = v;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map, buf, col, row0);
+    bulk_commit();
+  }
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const __grid_constant__ MxParams p) {
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+  uint64_t* full = bars;                    // TMA (both CTAs) -> MMA; used in rank 0
+  uint64_t* empty = bars + STAGES;          // MMA -> TMA, in each CTA
+  uint64_t* tmem_full = bars + 2 * STAGES;  // MMA -> epilogue, in each CTA (2)
+  uint64_t* tmem_free = tmem_full + 2;      // epilogues -> MMA; used in rank 0
+  uint64_t* mma_done = tmem_free + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const uint32_t warp = warp_id(), lane = lane_id();
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) mbar_init(&tmem_full[a], 1);
+    mbar_init(tmem_free, 8);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int num_kb = (p.K + kMxStageK - 1) / kMxStageK;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int num_units = sk_units(tiles, p.sk_tail, p.sk_split);
+  const int first_unit = static_cast<int>(cluster_id_x());
+  const int unit_step = static_cast<int>(num_clusters_x());
+  uint32_t* status = p.status;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&p.tmA);
+      tma_prefetch_desc(&p.tmB);
+      tma_prefetch_desc(&p.tmAs);
+      tma_prefetch_desc(&p.tmBs);
+      uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
+      bool ok = true;
+      for (int u = first_unit; u < num_units && ok; u += unit_step) {
+        const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+        int pm, pn;
+        tile_coords(w.tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
+        const int am = 2 * pm + static_cast<int>(rank);  // 128-row blocks of A and B of this CTA
+        const int bn = 2 * pn + static_cast<int>(rank);
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = smem + stage * Cfg::STAGE_BYTES;
+          const uint32_t bar = map_to_rank(&full[stage], 0);
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
+          tma_load_2d_pair(sa, &p.tmA, bar, kb * 128, am * 128);
+          tma_load_2d_pair(sa + Cfg::OPERAND_BYTES, &p.tmB, bar, kb * 128, bn * 128);
+          tma_load_2d_pair(sa + Cfg::SFA_OFFSET, &p.tmAs, bar, kb * 256, am);
+          // Every MMA reads the scales of all 256 columns in both CTAs.
+          tma_load_2d_pair(sa + Cfg::SFB_OFFSET, &p.tmBs, bar, kb * 256, 2 * pn);
+          tma_load_2d_pair(sa + Cfg::SFB_OFFSET + kMxScaleBytes, &p.tmBs, bar, kb * 256, 2 * pn + 1);
+          filled |= 1u << stage;
+          fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // Drain: a stage this CTA filled is finished once the MMA released it.
+      for (int s = 0; s < STAGES; ++s) {
+        if (filled & (1u << s)) {
+          volatile int never = 0;
+          mbar_wait(&empty[s], (fill_parity >> s) & 1u, &never, status, kErrTimeoutTeardown);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc[2] = {make_idesc_mxf4(256, 256, 0), make_idesc_mxf4(256, 256, 2)};
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      uint32_t old_stage = STAGES - 2, old_phase = 1;  // the k-block before the previous one
+      uint32_t sf = 0;
+      int issued = 0;  // k-blocks, up to 2
+      bool ok = true, first = true;
+      for (int u = first_unit; u < num_units && ok; u += unit_step) {
+        const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+        // The previous tile's epilogue has read the columns both accumulators
+        // share (and, before that, all of the tile before it).
+        if (!first) {
+          if (!mbar_wait(tmem_free, acc_phase, abort_flag, status, kErrTimeoutMma)) break;
+          tc_fence_after_sync();
+          acc_phase ^= 1;
+        }
+        first = false;
+        const uint32_t d_tmem = tmem_base + acc * Cfg::ACC_STEP;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!mbar_wait(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          if (issued >= 2 && !mbar_wait(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t sa = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+          const uint32_t sb = sa + Cfg::OPERAND_BYTES;
+          const uint32_t sfa = tmem_base + Cfg::SF_COL + 32 * sf, sfb = sfa + 8;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            tmem_cp_scales_pair(sfa + 4 * t, make_smem_desc_scales(sa + Cfg::SFA_OFFSET + t * kMxTileBytes));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tmem_cp_scales_pair(sfb + 8 * t + 4 * h, make_smem_desc_scales(sa + Cfg::SFB_OFFSET +
+                                                                             h * kMxScaleBytes + t * kMxTileBytes));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            umma_mxf4_ss_pair(d_tmem, make_smem_desc_sw128(sa + k * 32, 16, 1024),
+                              make_smem_desc_sw128(sb + k * 32, 16, 1024), idesc[k & 1], sfa + 4 * (k >> 1),
+                              sfb + 8 * (k >> 1), (kb != w.kb0 || k != 0) ? 1u : 0u);
+          }
+          umma_commit_pair(map_to_rank(&empty[stage], 0));
+          umma_commit_pair(map_to_rank(&empty[stage], 1));
+          if (issued < 2) ++issued;
+          if (++old_stage == STAGES) {
+            old_stage = 0;
+            old_phase ^= 1;
+          }
+          sf ^= 1;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        umma_commit_pair(map_to_rank(&tmem_full[acc], 0));
+        umma_commit_pair(map_to_rank(&tmem_full[acc], 1));
+        acc ^= 1;
+      }
+      umma_commit_pair(map_to_rank(mma_done, 0));
+      volatile int never = 0;
+      mbar_wait(mma_done, 0, &never, status, kErrTimeoutTeardown);
+    }
+  } else {
+    const uint32_t q = warp & 3u;
+    uint32_t acc = 0, acc_phase = 0;
+    uint8_t* stage = smem + Cfg::EPI_OFFSET + (warp - 2) * StoreStage<Cfg::OUT_F32>::kWarpBytes;
+    constexpr int kBufBytes = StoreStage<Cfg::OUT_F32>::kWarpBytes / 2;
+    auto free_acc = [&] {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_rank(tmem_free, 0));
+    };
+    for (int u = first_unit; u < num_units; u += unit_step) {
+      const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+      int pm, pn;
+      tile_coords(w.tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
+      if (!mbar_wait(&tmem_full[acc], acc_phase, abort_flag, status, kErrTimeoutEpilogue)) break;
+      tc_fence_after_sync();
+      const int row_in_tile = 128 * static_cast<int>(rank) + static_cast<int>(q * 32 + lane);
+      const int row0 = pm * 256 + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
+      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * Cfg::ACC_STEP;
+      bool mine = true, freed = false;
+      if (w.parts > 1) {
+        // A part of a split tile: the last to arrive for this 32-row slab
+        // finishes it. The sum is built in TMEM, so nothing is freed early.
+        const int i = w.tile - (tiles - p.sk_tail);
+        const long long part_stride = 256ll * 256;
+        const float* fix = p.sk_partials + (static_cast<long long>(i) * w.parts * 256 + row_in_tile) * 256;
+        mine = sk_publish_and_fix(t_row, 256, const_cast<float*>(fix) + w.part * part_stride, fix, part_stride,
+                                  w.parts, p.sk_counters + i * 8 + rank * 4 + q, 1);
+      }
+      if (mine) {
+        // Shared columns first: chunks 7, 6 of accumulator 0; 0, 1 of accumulator 1.
+        const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
+        uint32_t r[32], r2[32];
+        tmem_ld_32x32b_x32(t_row + c_first * 32, r);
+        tmem_ld_32x32b_x32(t_row + (c_first + c_step) * 32, r2);
+        tmem_ld_wait();
+        if (w.parts == 1) {
+          free_acc();
+          freed = true;
+        }
+        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r, stage, pn * 256 + c_first * 32, row0);
+        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r2, stage + kBufBytes, pn * 256 + (c_first + c_step) * 32, row0);
+#pragma unroll 1
+        for (int i = 2; i < 8; ++i) {
+          const int c = c_first + i * c_step;
+          tmem_ld_32x32b_x32(t_row + c * 32, r);
+          tmem_ld_wait();
+          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r, stage + (i & 1) * kBufBytes, pn * 256 + c * 32, row0);
+        }
+      }
+      if (!freed) free_acc();
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    // The TMA stores read shared memory asynchronously: finish before exit.
+    if (lane == 0) bulk_wait_read<0>();
+  }
+
+  // Neither CTA releases TMEM (or exits) before the pair is done with it.
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------ few rows
+// M <= 128: the roles are swapped. The tensor core's 128-row operand is a tile
+// of B (the weight), its columns are the M tokens padded to NT, so a weight
+// byte is loaded once and no part of a tile is wasted on rows that do not
+// exist. The work is the weight's bytes; when its tiles are fewer than the
+// CTAs that fit, a cluster of CTAs shares a tile and splits K, and the parts
+// are added in rank order through distributed shared memory.
+struct MxFewParams {
+  CUtensorMap tmW, tmWs;  // weight codes {128 bytes, 128 rows}, its scale tiles
+  CUtensorMap tmX, tmXs;  // token codes {128 bytes, NT rows}, their scale tiles
+  void* out;              // [M, N]
+  int M, N, K;
+  uint32_t* status;
+};
+
+template <int NT_, bool OUT_F32_>
+struct MxFewCfg {
+  static constexpr int NT = NT_;
+  static constexpr bool OUT_F32 = OUT_F32_;
+  static constexpr int W_BYTES = 128 * 128;
+  static constexpr int X_BYTES = NT * 128;
+  static constexpr int SFW_OFFSET = W_BYTES + X_BYTES;
+  static constexpr int SFX_OFFSET = SFW_OFFSET + kMxScaleBytes;
+  static constexpr int STAGE_BYTES = SFX_OFFSET + kMxScaleBytes;
+  // About 100 KB a CTA, two CTAs an SM: twice what the latency of HBM asks for.
+  static constexpr int STAGES = 100 * 1024 / STAGE_BYTES;
+  static constexpr int SF_COL = NT;  // scale buffers: 16 columns each
+  static constexpr int TMEM_COLS = NT + 32 <= 64 ? 64 : NT + 32 <= 128 ? 128 : 256;
+  static constexpr int NUM_THREADS = 192;
+  static constexpr int BAR_BYTES = 8 * (2 * STAGES + 1) + 16;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + BAR_BYTES;
+  static_assert(STAGES >= 2 && STAGES * STAGE_BYTES >= NT * 128 * 4, "the ring also holds the parts");
+  static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __grid_constant__ MxFewParams p) {
+  constexpr int STAGES = Cfg::STAGES, NT = Cfg::NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tmem_full = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const uint32_t warp = warp_id(), lane = lane_id();
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int parts = static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x());  // cluster size
+  const int tile = static_cast<int>(cluster_id_x());
+  const int num_kb = (p.K + kMxStageK - 1) / kMxStageK;
+  const int kb0 = rank * num_kb / parts, kb1 = (rank + 1) * num_kb / parts;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tmem_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  uint32_t* status = p.status;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) break;
+        uint8_t* s = smem + stage * Cfg::STAGE_BYTES;
+        mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
+        tma_load_2d(s, &p.tmW, &full[stage], kb * 128, tile * 128);
+        tma_load_2d(s + Cfg::SFW_OFFSET, &p.tmWs, &full[stage], kb * 256, tile);
+        tma_load_2d(s + Cfg::W_BYTES, &p.tmX, &full[stage], kb * 128, 0);
+        tma_load_2d(s + Cfg::SFX_OFFSET, &p.tmXs, &full[stage], kb * 256, 0);
+        filled |= 1u << stage;
+        fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      // Drain: every load this thread issued must land before the CTA exits.
+      for (int s = 0; s < STAGES; ++s) {
+        if (filled & (1u << s)) {
+          volatile int never = 0;
+          mbar_wait(&full[s], (fill_parity >> s) & 1u, &never, status, kErrTimeoutTeardown);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc[2] = {make_idesc_mxf4(128, NT, 0), make_idesc_mxf4(128, NT, 2)};
+      uint32_t stage = 0, phase = 0, old_stage = 0, old_phase = 0, sf = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) break;
+        if (kb >= kb0 + 2) {  // the MMAs that read this scale buffer last
+          if (!mbar_wait(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) break;
+          if (++old_stage == STAGES) {
+            old_stage = 0;
+            old_phase ^= 1;
+          }
+        }
+        tc_fence_after_sync();
+        const uint32_t sw = smem_u32(smem + stage * Cfg::STAGE_BYTES), sx = sw + Cfg::W_BYTES;
+        const uint32_t sfw = tmem_base + Cfg::SF_COL + 16 * sf, sfx = sfw + 8;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          tmem_cp_scales(sfw + 4 * t, make_smem_desc_scales(sw + Cfg::SFW_OFFSET + t * kMxTileBytes));
+          tmem_cp_scales(sfx + 4 * t, make_smem_desc_scales(sw + Cfg::SFX_OFFSET + t * kMxTileBytes));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          umma_mxf4_ss(tmem_base, make_smem_desc_sw128(sw + k * 32, 16, 1024),
+                       make_smem_desc_sw128(sx + k * 32, 16, 1024), idesc[k & 1], sfw + 4 * (k >> 1),
+                       sfx + 4 * (k >> 1), (kb != kb0 || k != 0) ? 1u : 0u);
+        }
+        umma_commit(&empty[stage]);
+        sf ^= 1;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      umma_commit(tmem_full);  // arrives when all MMAs issued so far are done
+      volatile int never = 0;
+      mbar_wait(tmem_full, 0, &never, status, kErrTimeoutTeardown);
+    }
+  }
+
+  // Output of one token and weight row.
+  auto store = [&](int token, int row, float v) {
+    const long long at = static_cast<long long>(token) * p.N + tile * 128ll + row;
+    if (tile * 128 + row < p.N) {
+      if constexpr (Cfg::OUT_F32) static_cast<float*>(p.out)[at] = v;
+      else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    }
+  };
+  const int row = static_cast<int>((warp & 3u) * 32 + lane);  // TMEM lane = weight row (warps 2..5)
+  float* part = reinterpret_cast<float*>(smem);               // [NT][128], over the ring once its MMAs are done
+  bool ok = true;
+  if (warp >= 2) {
+    ok = mbar_wait(tmem_full, 0, abort_flag, status, kErrTimeoutEpilogue);
+    if (ok) {
+      tc_fence_after_sync();
+      const uint32_t t_row = tmem_base + (((warp & 3u) * 32u) << 16);
+#pragma unroll
+      for (int c = 0; c < NT; c += 16) {
+        if (c >= p.M) break;
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(t_row + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (c + i < p.M) {
+            if (parts == 1) store(c + i, row, __uint_as_float(r[i]));
+            else part[(c + i) * 128 + row] = __uint_as_float(r[i]);
+          }
+        }
+      }
+    }
+  }
+  if (parts > 1) {
+    cluster_sync_all();
+    if (warp >= 2 && ok) {
+      for (int t = rank; t < p.M; t += parts) {
+        float v = 0.0f;
+        for (int s = 0; s < parts; ++s) v += ld_cluster_f32(map_to_rank(&part[t * 128 + row], s));
+        store(t, row, v);
+      }
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its parts
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace swiglu

@@ -65,7 +65,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         subprocess.run(cmd, check=True, stdout=None if verbose else subprocess.PIPE,
                        stderr=subprocess.STDOUT if not verbose else None)
     except subprocess.CalledProcessError as e:
-        os.unlink(tmp)
+        if os.path.exists(tmp):
+            os.unlink(tmp)
         out = e.stdout.decode(errors="replace") if e.stdout else ""
         raise RuntimeError(f"nvcc failed:\n{out}") from None
     os.replace(tmp, LIB_PATH)
