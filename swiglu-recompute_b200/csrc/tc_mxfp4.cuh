@@ -5,8 +5,15 @@
 // (128-byte swizzle, as the 8- and 16-bit kernels) and the scale tiles of the
 // same rows: two tiles of 512 bytes per 128 rows, copied by the MMA thread to
 // TMEM (tcgen05.cp) right before the four MMAs (K = 64 each) that use them.
-// Scale columns are double-buffered: the copy for k-block i waits for the MMAs
-// of k-block i - 2, so it runs under those of i - 1.
+// The copies and the MMAs of a thread run in order, so a copy issued right
+// before the MMAs that need it leaves the tensor core idle for its latency: the
+// copies for k-block i + 1 are issued before the MMAs of k-block i.
+//
+// The TMA and MMA roles run as whole warps that elect a lane for the
+// instructions (elect.sync): from code that only lane 0 enters, each tcgen05
+// instruction took about 65 cycles to issue (11136 x 28672 x 3584: 646 us; the
+// loads and the number of stages made no difference), half again what its
+// work takes here, where an MMA is four times as short as for 16-bit operands.
 //
 // Out-of-range rows, columns of K and scale tiles are filled with zeros by TMA:
 // a zero code times 2^-127 is zero, so no tail needs a case of its own.
@@ -34,8 +41,8 @@ struct MxParams {
   int sk_tail, sk_split;
 };
 
-// TMEM: two 256-column accumulators that share 64 columns (0..255 and
-// 192..447) leave 64 columns for the scales. The epilogue reads the shared
+// TMEM: two 256-column accumulators that share 96 columns (0..255 and
+// 160..415) leave 96 columns for four buffers of scales. The epilogue reads the shared
 // columns first and frees them, then the next tile's MMAs may start: with two
 // whole accumulators TMEM would be full.
 template <bool OUT_F32_>
@@ -46,12 +53,14 @@ struct MxCfg {
   static constexpr int SFA_OFFSET = 2 * OPERAND_BYTES;
   static constexpr int SFB_OFFSET = SFA_OFFSET + kMxScaleBytes;
   static constexpr int STAGE_BYTES = SFB_OFFSET + 2 * kMxScaleBytes;
-  static constexpr int ACC_STEP = 192;  // accumulator 1 starts here
-  static constexpr int SF_COL = 448;    // scale buffers: 448 and 480, 24 columns each
+  static constexpr int ACC_STEP = 160;  // accumulator 1 starts here
+  static constexpr int SF_COL = 416;    // scale buffers, 24 columns each
+  static constexpr int SF_BUFS = 4;
   static constexpr int NUM_THREADS = 192;
   static constexpr int BAR_BYTES = 8 * (2 * STAGES + 4) + 16;
   static constexpr int EPI_OFFSET = STAGES * STAGE_BYTES + ((BAR_BYTES + 1023) / 1024) * 1024;
   static constexpr int SMEM_BYTES = 1024 + EPI_OFFSET + 4 * StoreStage<OUT_F32>::kWarpBytes;
+  static_assert(SF_BUFS <= STAGES, "a stage's MMAs of SF_BUFS k-blocks ago are awaited by its phase");
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
@@ -134,24 +143,20 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
   uint32_t* status = p.status;
 
   if (warp == 0) {
-    if (lane == 0) {
-      tma_prefetch_desc(&p.tmA);
-      tma_prefetch_desc(&p.tmB);
-      tma_prefetch_desc(&p.tmAs);
-      tma_prefetch_desc(&p.tmBs);
-      uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
-      bool ok = true;
-      for (int u = first_unit; u < num_units && ok; u += unit_step) {
-        const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
-        int pm, pn;
-        tile_coords(w.tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
-        const int am = 2 * pm + static_cast<int>(rank);  // 128-row blocks of A and B of this CTA
-        const int bn = 2 * pn + static_cast<int>(rank);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) {
-            ok = false;
-            break;
-          }
+    uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
+    bool ok = true;
+    for (int u = first_unit; u < num_units && ok; u += unit_step) {
+      const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+      int pm, pn;
+      tile_coords(w.tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
+      const int am = 2 * pm + static_cast<int>(rank);  // 128-row blocks of A and B of this CTA
+      const int bn = 2 * pn + static_cast<int>(rank);
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
           uint8_t* sa = smem + stage * Cfg::STAGE_BYTES;
           const uint32_t bar = map_to_rank(&full[stage], 0);
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
@@ -161,89 +166,121 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
           // Every MMA reads the scales of all 256 columns in both CTAs.
           tma_load_2d_pair(sa + Cfg::SFB_OFFSET, &p.tmBs, bar, kb * 256, 2 * pn);
           tma_load_2d_pair(sa + Cfg::SFB_OFFSET + kMxScaleBytes, &p.tmBs, bar, kb * 256, 2 * pn + 1);
-          filled |= 1u << stage;
-          fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
-      }
-      // Drain: a stage this CTA filled is finished once the MMA released it.
-      for (int s = 0; s < STAGES; ++s) {
-        if (filled & (1u << s)) {
-          volatile int never = 0;
-          mbar_wait(&empty[s], (fill_parity >> s) & 1u, &never, status, kErrTimeoutTeardown);
+        __syncwarp();
+        filled |= 1u << stage;
+        fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
         }
       }
     }
+    // Drain: a stage this CTA filled is finished once the MMA released it.
+    for (int s = 0; s < STAGES; ++s) {
+      if (filled & (1u << s)) {
+        volatile int never = 0;
+        mbar_wait_warp(&empty[s], (fill_parity >> s) & 1u, &never, status, kErrTimeoutTeardown);
+      }
+    }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       constexpr uint32_t idesc[2] = {make_idesc_mxf4(256, 256, 0), make_idesc_mxf4(256, 256, 2)};
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      uint32_t old_stage = STAGES - 2, old_phase = 1;  // the k-block before the previous one
-      uint32_t sf = 0;
-      int issued = 0;  // k-blocks, up to 2
+      const uint32_t smem0 = smem_u32(smem);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, sf = 0;
+      // The next k-block whose scales are to be copied, and the one whose MMAs
+      // used that scale buffer last.
+      uint32_t cp_stage = 0, cp_phase = 0, cp_sf = 0, old_stage = 0, old_phase = 0;
+      int copied = 0;      // k-blocks copied so far, up to SF_BUFS
+      bool ahead = false;  // the scales of the current k-block are already copied
       bool ok = true, first = true;
+      auto copy_scales = [&]() -> bool {  // full[cp_stage] has completed
+        if (copied == Cfg::SF_BUFS) {
+          if (!mbar_wait_warp(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) return false;
+          if (++old_stage == STAGES) {
+            old_stage = 0;
+            old_phase ^= 1;
+          }
+        } else {
+          ++copied;
+        }
+        tc_fence_after_sync();
+        const uint32_t s = smem0 + cp_stage * Cfg::STAGE_BYTES;
+        const uint32_t sfa = tmem_base + Cfg::SF_COL + 24 * cp_sf, sfb = sfa + 8;
+        if (elect_one()) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            tmem_cp_scales_pair(sfa + 4 * t, make_smem_desc_scales(s + Cfg::SFA_OFFSET + t * kMxTileBytes));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tmem_cp_scales_pair(sfb + 8 * t + 4 * h,
+                                  make_smem_desc_scales(s + Cfg::SFB_OFFSET + h * kMxScaleBytes + t * kMxTileBytes));
+          }
+        }
+        __syncwarp();
+        cp_sf = cp_sf + 1 == Cfg::SF_BUFS ? 0 : cp_sf + 1;
+        if (++cp_stage == STAGES) {
+          cp_stage = 0;
+          cp_phase ^= 1;
+        }
+        return true;
+      };
       for (int u = first_unit; u < num_units && ok; u += unit_step) {
         const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
         // The previous tile's epilogue has read the columns both accumulators
         // share (and, before that, all of the tile before it).
         if (!first) {
-          if (!mbar_wait(tmem_free, acc_phase, abort_flag, status, kErrTimeoutMma)) break;
+          if (!mbar_wait_warp(tmem_free, acc_phase, abort_flag, status, kErrTimeoutMma)) break;
           tc_fence_after_sync();
           acc_phase ^= 1;
         }
         first = false;
         const uint32_t d_tmem = tmem_base + acc * Cfg::ACC_STEP;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) {
-            ok = false;
-            break;
+          if (!ahead) {
+            if (!mbar_wait_warp(&full[stage], phase, abort_flag, status, kErrTimeoutMma) || !copy_scales()) {
+              ok = false;
+              break;
+            }
           }
-          if (issued >= 2 && !mbar_wait(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) {
+          // The next k-block's scales, if it has arrived; else after the wait above.
+          ahead = (kb + 1 < w.kb1 || u + unit_step < num_units) &&
+                  __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&full[cp_stage]), cp_phase));
+          if (ahead && !copy_scales()) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t sa = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+          const uint32_t sa = smem0 + stage * Cfg::STAGE_BYTES;
           const uint32_t sb = sa + Cfg::OPERAND_BYTES;
-          const uint32_t sfa = tmem_base + Cfg::SF_COL + 32 * sf, sfb = sfa + 8;
+          const uint32_t sfa = tmem_base + Cfg::SF_COL + 24 * sf, sfb = sfa + 8;
+          if (elect_one()) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            tmem_cp_scales_pair(sfa + 4 * t, make_smem_desc_scales(sa + Cfg::SFA_OFFSET + t * kMxTileBytes));
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              tmem_cp_scales_pair(sfb + 8 * t + 4 * h, make_smem_desc_scales(sa + Cfg::SFB_OFFSET +
-                                                                             h * kMxScaleBytes + t * kMxTileBytes));
+            for (int k = 0; k < 4; ++k) {
+              umma_mxf4_ss_pair(d_tmem, make_smem_desc_sw128(sa + k * 32, 16, 1024),
+                                make_smem_desc_sw128(sb + k * 32, 16, 1024), idesc[k & 1], sfa + 4 * (k >> 1),
+                                sfb + 8 * (k >> 1), (kb != w.kb0 || k != 0) ? 1u : 0u);
+            }
+            umma_commit_pair(map_to_rank(&empty[stage], 0));
+            umma_commit_pair(map_to_rank(&empty[stage], 1));
+            if (kb + 1 == w.kb1) {
+              umma_commit_pair(map_to_rank(&tmem_full[acc], 0));
+              umma_commit_pair(map_to_rank(&tmem_full[acc], 1));
+            }
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            umma_mxf4_ss_pair(d_tmem, make_smem_desc_sw128(sa + k * 32, 16, 1024),
-                              make_smem_desc_sw128(sb + k * 32, 16, 1024), idesc[k & 1], sfa + 4 * (k >> 1),
-                              sfb + 8 * (k >> 1), (kb != w.kb0 || k != 0) ? 1u : 0u);
-          }
-          umma_commit_pair(map_to_rank(&empty[stage], 0));
-          umma_commit_pair(map_to_rank(&empty[stage], 1));
-          if (issued < 2) ++issued;
-          if (++old_stage == STAGES) {
-            old_stage = 0;
-            old_phase ^= 1;
-          }
-          sf ^= 1;
+          __syncwarp();
+          sf = sf + 1 == Cfg::SF_BUFS ? 0 : sf + 1;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (!ok) break;
-        umma_commit_pair(map_to_rank(&tmem_full[acc], 0));
-        umma_commit_pair(map_to_rank(&tmem_full[acc], 1));
         acc ^= 1;
       }
-      umma_commit_pair(map_to_rank(mma_done, 0));
+      if (elect_one()) umma_commit_pair(map_to_rank(mma_done, 0));
+      __syncwarp();
       volatile int never = 0;
-      mbar_wait(mma_done, 0, &never, status, kErrTimeoutTeardown);
+      mbar_wait_warp(mma_done, 0, &never, status, kErrTimeoutTeardown);
     }
   } else {
     const uint32_t q = warp & 3u;
@@ -275,20 +312,22 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
                                   w.parts, p.sk_counters + i * 8 + rank * 4 + q, 1);
       }
       if (mine) {
-        // Shared columns first: chunks 7, 6 of accumulator 0; 0, 1 of accumulator 1.
+        // Shared columns first: chunks 7, 6, 5 of accumulator 0; 0, 1, 2 of accumulator 1.
         const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
-        uint32_t r[32], r2[32];
+        uint32_t r[32], r1[32], r2[32];
         tmem_ld_32x32b_x32(t_row + c_first * 32, r);
-        tmem_ld_32x32b_x32(t_row + (c_first + c_step) * 32, r2);
+        tmem_ld_32x32b_x32(t_row + (c_first + c_step) * 32, r1);
+        tmem_ld_32x32b_x32(t_row + (c_first + 2 * c_step) * 32, r2);
         tmem_ld_wait();
         if (w.parts == 1) {
           free_acc();
           freed = true;
         }
         mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r, stage, pn * 256 + c_first * 32, row0);
-        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r2, stage + kBufBytes, pn * 256 + (c_first + c_step) * 32, row0);
+        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r1, stage + kBufBytes, pn * 256 + (c_first + c_step) * 32, row0);
+        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r2, stage, pn * 256 + (c_first + 2 * c_step) * 32, row0);
 #pragma unroll 1
-        for (int i = 2; i < 8; ++i) {
+        for (int i = 3; i < 8; ++i) {
           const int c = c_first + i * c_step;
           tmem_ld_32x32b_x32(t_row + c * 32, r);
           tmem_ld_wait();
@@ -392,47 +431,48 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
   uint32_t* status = p.status;
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) break;
+    uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) break;
+      if (elect_one()) {
         uint8_t* s = smem + stage * Cfg::STAGE_BYTES;
         mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
         tma_load_2d(s, &p.tmW, &full[stage], kb * 128, tile * 128);
         tma_load_2d(s + Cfg::SFW_OFFSET, &p.tmWs, &full[stage], kb * 256, tile);
         tma_load_2d(s + Cfg::W_BYTES, &p.tmX, &full[stage], kb * 128, 0);
         tma_load_2d(s + Cfg::SFX_OFFSET, &p.tmXs, &full[stage], kb * 256, 0);
-        filled |= 1u << stage;
-        fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      // Drain: every load this thread issued must land before the CTA exits.
-      for (int s = 0; s < STAGES; ++s) {
-        if (filled & (1u << s)) {
-          volatile int never = 0;
-          mbar_wait(&full[s], (fill_parity >> s) & 1u, &never, status, kErrTimeoutTeardown);
-        }
+      __syncwarp();
+      filled |= 1u << stage;
+      fill_parity = (fill_parity & ~(1u << stage)) | (phase << stage);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    // Drain: every load this warp issued must land before the CTA exits.
+    for (int s = 0; s < STAGES; ++s) {
+      if (filled & (1u << s)) {
+        volatile int never = 0;
+        mbar_wait_warp(&full[s], (fill_parity >> s) & 1u, &never, status, kErrTimeoutTeardown);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc[2] = {make_idesc_mxf4(128, NT, 0), make_idesc_mxf4(128, NT, 2)};
-      uint32_t stage = 0, phase = 0, old_stage = 0, old_phase = 0, sf = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) break;
-        if (kb >= kb0 + 2) {  // the MMAs that read this scale buffer last
-          if (!mbar_wait(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) break;
-          if (++old_stage == STAGES) {
-            old_stage = 0;
-            old_phase ^= 1;
-          }
+    constexpr uint32_t idesc[2] = {make_idesc_mxf4(128, NT, 0), make_idesc_mxf4(128, NT, 2)};
+    uint32_t stage = 0, phase = 0, old_stage = 0, old_phase = 0, sf = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) break;
+      if (kb >= kb0 + 2) {  // the MMAs that read this scale buffer last
+        if (!mbar_wait_warp(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) break;
+        if (++old_stage == STAGES) {
+          old_stage = 0;
+          old_phase ^= 1;
         }
-        tc_fence_after_sync();
-        const uint32_t sw = smem_u32(smem + stage * Cfg::STAGE_BYTES), sx = sw + Cfg::W_BYTES;
-        const uint32_t sfw = tmem_base + Cfg::SF_COL + 16 * sf, sfx = sfw + 8;
+      }
+      tc_fence_after_sync();
+      const uint32_t sw = smem_u32(smem + stage * Cfg::STAGE_BYTES), sx = sw + Cfg::W_BYTES;
+      const uint32_t sfw = tmem_base + Cfg::SF_COL + 16 * sf, sfx = sfw + 8;
+      if (elect_one()) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           tmem_cp_scales(sfw + 4 * t, make_smem_desc_scales(sw + Cfg::SFW_OFFSET + t * kMxTileBytes));
@@ -445,16 +485,18 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
                        sfx + 4 * (k >> 1), (kb != kb0 || k != 0) ? 1u : 0u);
         }
         umma_commit(&empty[stage]);
-        sf ^= 1;
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      umma_commit(tmem_full);  // arrives when all MMAs issued so far are done
-      volatile int never = 0;
-      mbar_wait(tmem_full, 0, &never, status, kErrTimeoutTeardown);
+      __syncwarp();
+      sf ^= 1;
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
+    if (elect_one()) umma_commit(tmem_full);  // arrives when all MMAs issued so far are done
+    __syncwarp();
+    volatile int never = 0;
+    mbar_wait_warp(tmem_full, 0, &never, status, kErrTimeoutTeardown);
   }
 
   // Output of one token and weight row.
