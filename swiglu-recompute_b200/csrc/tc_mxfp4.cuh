@@ -3,17 +3,17 @@
 //
 // Per k-block of 256 elements a stage holds 128 bytes of each operand row
 // (128-byte swizzle, as the 8- and 16-bit kernels) and the scale tiles of the
-// same rows: two tiles of 512 bytes per 128 rows, copied by the MMA thread to
-// TMEM (tcgen05.cp) right before the four MMAs (K = 64 each) that use them.
-// The copies and the MMAs of a thread run in order, so a copy issued right
-// before the MMAs that need it leaves the tensor core idle for its latency: the
-// copies for k-block i + 1 are issued before the MMAs of k-block i.
+// same rows: two tiles of 512 bytes per 128 rows, copied to TMEM (tcgen05.cp)
+// for the four MMAs (K = 64 each) of the k-block.
 //
-// The TMA and MMA roles run as whole warps that elect a lane for the
-// instructions (elect.sync): from code that only lane 0 enters, each tcgen05
-// instruction took about 65 cycles to issue (11136 x 28672 x 3584: 646 us; the
-// loads and the number of stages made no difference), half again what its
-// work takes here, where an MMA is four times as short as for 16-bit operands.
+// An MMA is four times as short here as for 16-bit operands, so what bounds the
+// product is how fast the k-blocks are issued (11136 x 28672 x 3584, one box):
+//   one lane of one warp waits, copies scales and issues MMAs   646 us
+//     (without the copies 460, one MMA of four 530; half the loads, fewer
+//     stages or no stores: no change)
+//   whole warps, a lane elected for the instructions            485 us
+//     (without the copies 413, without waiting for a scale buffer 50 less)
+//   MXP_RESULT
 //
 // Out-of-range rows, columns of K and scale tiles are filled with zeros by TMA:
 // a zero code times 2^-127 is zero, so no tail needs a case of its own.
@@ -41,10 +41,11 @@ struct MxParams {
   int sk_tail, sk_split;
 };
 
-// TMEM: two 256-column accumulators that share 96 columns (0..255 and
-// 160..415) leave 96 columns for four buffers of scales. The epilogue reads the shared
-// columns first and frees them, then the next tile's MMAs may start: with two
-// whole accumulators TMEM would be full.
+// TMEM: two 256-column accumulators that share 120 columns (0..255 and
+// 136..391) leave 120 columns for scales, one buffer of 24 per stage of the
+// ring, so that a stage's arrival also says that its scale buffer is free. The
+// epilogue reads the shared columns first and frees them, then the next tile's
+// MMAs may start: with two whole accumulators TMEM would be full.
 template <bool OUT_F32_>
 struct MxCfg {
   static constexpr bool OUT_F32 = OUT_F32_;
@@ -53,14 +54,13 @@ struct MxCfg {
   static constexpr int SFA_OFFSET = 2 * OPERAND_BYTES;
   static constexpr int SFB_OFFSET = SFA_OFFSET + kMxScaleBytes;
   static constexpr int STAGE_BYTES = SFB_OFFSET + 2 * kMxScaleBytes;
-  static constexpr int ACC_STEP = 160;  // accumulator 1 starts here
-  static constexpr int SF_COL = 416;    // scale buffers, 24 columns each
-  static constexpr int SF_BUFS = 4;
-  static constexpr int NUM_THREADS = 192;
-  static constexpr int BAR_BYTES = 8 * (2 * STAGES + 4) + 16;
+  static constexpr int ACC_STEP = 136;             // accumulator 1 starts here
+  static constexpr int SF_COL = ACC_STEP + 256;    // scale buffers, 24 columns a stage
+  static constexpr int NUM_THREADS = 224;
+  static constexpr int BAR_BYTES = 8 * (3 * STAGES + 5) + 16;
   static constexpr int EPI_OFFSET = STAGES * STAGE_BYTES + ((BAR_BYTES + 1023) / 1024) * 1024;
   static constexpr int SMEM_BYTES = 1024 + EPI_OFFSET + 4 * StoreStage<OUT_F32>::kWarpBytes;
-  static_assert(SF_BUFS <= STAGES, "a stage's MMAs of SF_BUFS k-blocks ago are awaited by its phase");
+  static_assert(SF_COL + 24 * STAGES <= 512, "TMEM holds 512 columns");
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
@@ -105,10 +105,12 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
   uint64_t* full = bars;                    // TMA (both CTAs) -> MMA; used in rank 0
   uint64_t* empty = bars + STAGES;          // MMA -> TMA, in each CTA
-  uint64_t* tmem_full = bars + 2 * STAGES;  // MMA -> epilogue, in each CTA (2)
+  uint64_t* scaled = bars + 2 * STAGES;     // scale copies -> MMA; used in rank 0
+  uint64_t* tmem_full = bars + 3 * STAGES;  // MMA -> epilogue, in each CTA (2)
   uint64_t* tmem_free = tmem_full + 2;      // epilogues -> MMA; used in rank 0
   uint64_t* mma_done = tmem_free + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* copies_done = mma_done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(copies_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const uint32_t warp = warp_id(), lane = lane_id();
@@ -119,10 +121,12 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&scaled[s], 1);
     }
     for (int a = 0; a < 2; ++a) mbar_init(&tmem_full[a], 1);
     mbar_init(tmem_free, 8);
     mbar_init(mma_done, 1);
+    mbar_init(copies_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -187,73 +191,24 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
     if (leader) {
       constexpr uint32_t idesc[2] = {make_idesc_mxf4(256, 256, 0), make_idesc_mxf4(256, 256, 2)};
       const uint32_t smem0 = smem_u32(smem);
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0, sf = 0;
-      // The next k-block whose scales are to be copied, and the one whose MMAs
-      // used that scale buffer last.
-      uint32_t cp_stage = 0, cp_phase = 0, cp_sf = 0, old_stage = 0, old_phase = 0;
-      int copied = 0;      // k-blocks copied so far, up to SF_BUFS
-      bool ahead = false;  // the scales of the current k-block are already copied
-      bool ok = true, first = true;
-      auto copy_scales = [&]() -> bool {  // full[cp_stage] has completed
-        if (copied == Cfg::SF_BUFS) {
-          if (!mbar_wait_warp(&empty[old_stage], old_phase, abort_flag, status, kErrTimeoutMma)) return false;
-          if (++old_stage == STAGES) {
-            old_stage = 0;
-            old_phase ^= 1;
-          }
-        } else {
-          ++copied;
-        }
-        tc_fence_after_sync();
-        const uint32_t s = smem0 + cp_stage * Cfg::STAGE_BYTES;
-        const uint32_t sfa = tmem_base + Cfg::SF_COL + 24 * cp_sf, sfb = sfa + 8;
-        if (elect_one()) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            tmem_cp_scales_pair(sfa + 4 * t, make_smem_desc_scales(s + Cfg::SFA_OFFSET + t * kMxTileBytes));
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              tmem_cp_scales_pair(sfb + 8 * t + 4 * h,
-                                  make_smem_desc_scales(s + Cfg::SFB_OFFSET + h * kMxScaleBytes + t * kMxTileBytes));
-          }
-        }
-        __syncwarp();
-        cp_sf = cp_sf + 1 == Cfg::SF_BUFS ? 0 : cp_sf + 1;
-        if (++cp_stage == STAGES) {
-          cp_stage = 0;
-          cp_phase ^= 1;
-        }
-        return true;
-      };
+      uint32_t stage = 0, phase = 0, acc = 0, free_phase = 1;
+      bool ok = true;
       for (int u = first_unit; u < num_units && ok; u += unit_step) {
         const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
         // The previous tile's epilogue has read the columns both accumulators
         // share (and, before that, all of the tile before it).
-        if (!first) {
-          if (!mbar_wait_warp(tmem_free, acc_phase, abort_flag, status, kErrTimeoutMma)) break;
-          tc_fence_after_sync();
-          acc_phase ^= 1;
-        }
-        first = false;
+        if (!mbar_wait_warp(tmem_free, free_phase, abort_flag, status, kErrTimeoutMma)) break;
+        free_phase ^= 1;
         const uint32_t d_tmem = tmem_base + acc * Cfg::ACC_STEP;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!ahead) {
-            if (!mbar_wait_warp(&full[stage], phase, abort_flag, status, kErrTimeoutMma) || !copy_scales()) {
-              ok = false;
-              break;
-            }
-          }
-          // The next k-block's scales, if it has arrived; else after the wait above.
-          ahead = (kb + 1 < w.kb1 || u + unit_step < num_units) &&
-                  __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&full[cp_stage]), cp_phase));
-          if (ahead && !copy_scales()) {
+          if (!mbar_wait_warp(&scaled[stage], phase, abort_flag, status, kErrTimeoutMma)) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
           const uint32_t sa = smem0 + stage * Cfg::STAGE_BYTES;
           const uint32_t sb = sa + Cfg::OPERAND_BYTES;
-          const uint32_t sfa = tmem_base + Cfg::SF_COL + 24 * sf, sfb = sfa + 8;
+          const uint32_t sfa = tmem_base + Cfg::SF_COL + 24 * stage, sfb = sfa + 8;
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -261,15 +216,10 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
                                 make_smem_desc_sw128(sb + k * 32, 16, 1024), idesc[k & 1], sfa + 4 * (k >> 1),
                                 sfb + 8 * (k >> 1), (kb != w.kb0 || k != 0) ? 1u : 0u);
             }
-            umma_commit_pair(map_to_rank(&empty[stage], 0));
-            umma_commit_pair(map_to_rank(&empty[stage], 1));
-            if (kb + 1 == w.kb1) {
-              umma_commit_pair(map_to_rank(&tmem_full[acc], 0));
-              umma_commit_pair(map_to_rank(&tmem_full[acc], 1));
-            }
+            umma_commit_pair_both(&empty[stage]);
+            if (kb + 1 == w.kb1) umma_commit_pair_both(&tmem_full[acc]);
           }
           __syncwarp();
-          sf = sf + 1 == Cfg::SF_BUFS ? 0 : sf + 1;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -281,6 +231,47 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
       __syncwarp();
       volatile int never = 0;
       mbar_wait_warp(mma_done, 0, &never, status, kErrTimeoutTeardown);
+    }
+  } else if (warp == 6) {
+    // Scale tiles of each stage to TMEM. The stage arrived, so its previous
+    // MMAs, the last readers of its scale buffer, are done.
+    if (leader) {
+      const uint32_t smem0 = smem_u32(smem);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int u = first_unit; u < num_units && ok; u += unit_step) {
+        const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!mbar_wait_warp(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t s = smem0 + stage * Cfg::STAGE_BYTES;
+          const uint32_t sfa = tmem_base + Cfg::SF_COL + 24 * stage, sfb = sfa + 8;
+          if (elect_one()) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              tmem_cp_scales_pair(sfa + 4 * t, make_smem_desc_scales(s + Cfg::SFA_OFFSET + t * kMxTileBytes));
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                tmem_cp_scales_pair(sfb + 8 * t + 4 * h,
+                                    make_smem_desc_scales(s + Cfg::SFB_OFFSET + h * kMxScaleBytes + t * kMxTileBytes));
+            }
+            umma_commit_pair(map_to_rank(&scaled[stage], 0));
+          }
+          __syncwarp();
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // The copies read shared memory and write TMEM: none outlives this warp.
+      if (elect_one()) umma_commit_pair(map_to_rank(copies_done, 0));
+      __syncwarp();
+      volatile int never = 0;
+      mbar_wait_warp(copies_done, 0, &never, status, kErrTimeoutTeardown);
     }
   } else {
     const uint32_t q = warp & 3u;
@@ -312,27 +303,27 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
                                   w.parts, p.sk_counters + i * 8 + rank * 4 + q, 1);
       }
       if (mine) {
-        // Shared columns first: chunks 7, 6, 5 of accumulator 0; 0, 1, 2 of accumulator 1.
+        // Shared columns first: chunks 7..4 of accumulator 0, 0..3 of accumulator 1.
         const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
-        uint32_t r[32], r1[32], r2[32];
-        tmem_ld_32x32b_x32(t_row + c_first * 32, r);
-        tmem_ld_32x32b_x32(t_row + (c_first + c_step) * 32, r1);
-        tmem_ld_32x32b_x32(t_row + (c_first + 2 * c_step) * 32, r2);
+        uint32_t r[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + i * c_step) * 32, r[i]);
         tmem_ld_wait();
         if (w.parts == 1) {
           free_acc();
           freed = true;
         }
-        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r, stage, pn * 256 + c_first * 32, row0);
-        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r1, stage + kBufBytes, pn * 256 + (c_first + c_step) * 32, row0);
-        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r2, stage, pn * 256 + (c_first + 2 * c_step) * 32, row0);
-#pragma unroll 1
-        for (int i = 3; i < 8; ++i) {
-          const int c = c_first + i * c_step;
-          tmem_ld_32x32b_x32(t_row + c * 32, r);
-          tmem_ld_wait();
-          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r, stage + (i & 1) * kBufBytes, pn * 256 + c * 32, row0);
-        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
+                                       pn * 256 + (c_first + i * c_step) * 32, row0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + (4 + i) * c_step) * 32, r[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
+                                       pn * 256 + (c_first + (4 + i) * c_step) * 32, row0);
       }
       if (!freed) free_acc();
       acc ^= 1;
