@@ -347,14 +347,10 @@ int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, in
 
 /* C [M, N] = A . B^T for MXFP4 A [M, K] and B [N, K] with their scales, f32
  * accumulation, C in out_dtype. K % 32 == 0, N % 8 == 0; the MXFP4 form of
- * swiglu_b200_matmul_e4m3. workspace: 16-byte aligned device memory of the size
- * the query gives for a device with num_sms SMs (0: none needed), free for
- * other use once the call's work on the stream is done. The sums' order depends
- * on the sizes and the device (and swiglu_b200_set_sm_reserve) alone. */
-int swiglu_b200_matmul_mxfp4_workspace(int64_t M, int64_t N, int64_t K, int num_sms, int64_t* bytes);
+ * swiglu_b200_matmul_e4m3. From one row of A up; the sums' order depends on the
+ * sizes and the device (and swiglu_b200_set_sm_reserve) alone. */
 int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
-                             int64_t M, int64_t N, int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes,
-                             void* stream);
+                             int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
 
 /* Whole forward of one MLP block: preact (saved for backward), h (caller's
  * transient workspace [M, H]) and y [M, Dout].

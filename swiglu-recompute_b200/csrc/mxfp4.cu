@@ -248,43 +248,23 @@ int make_map_scales(CUtensorMap* m, const void* ptr, int64_t rows, int64_t K, co
   return SWIGLU_OK;
 }
 
-// How a product runs. few: the swapped kernel, `parts` CTAs of a cluster along
-// K per tile of 128 weight rows. Otherwise pair tiles, the last `tail` of them
-// split into `split` ranges of K, with `bytes` of workspace (arrival counters,
-// then the parts).
+// How a product runs: on 256 x 256 pair tiles, or on 128 x nt tiles with
+// clusters of `parts` CTAs along K.
 struct MxPlan {
-  bool few;
-  int parts;
-  int tiles_m, tiles_n, tail, split;
-  size_t bytes;
+  bool pair;
+  int nt, parts;
 };
-constexpr int kFewRows = 128;
-constexpr size_t kMxCounterBytes = 4096;
 
 MxPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
-  MxPlan p{};
-  const int num_kb = static_cast<int>((K + kMxStageK - 1) / kMxStageK);
-  p.split = p.parts = 1;
-  if (M <= kFewRows) {
-    p.few = true;
-    // Clusters as long as all CTAs fit at once, two to an SM.
-    const int64_t tiles = (N + 127) / 128;
-    while (p.parts < 8 && 2 * p.parts * tiles <= 2 * sms && 2 * p.parts <= num_kb) p.parts *= 2;
+  MxPlan p{false, 128, 1};
+  if (M > 128 && (M + 255) / 256 * ((N + 255) / 256) >= sms / 2) {
+    p.pair = true;
     return p;
   }
-  p.tiles_m = static_cast<int>((M + 255) / 256);
-  p.tiles_n = static_cast<int>((N + 255) / 256);
-  const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n, pairs = sms / 2 > 0 ? sms / 2 : 1;
-  const int64_t tail = tiles % pairs, rounds = (tiles + pairs - 1) / pairs;
-  // As the 2-SM kernels: only where a split saves 5 % of the pairs' rounds.
-  if (tail == 0 || (pairs - tail) * 20 < pairs * rounds) return p;
-  int64_t split = pairs / tail;
-  if (split > 16) split = 16;
-  if (split > num_kb / 4) split = num_kb / 4;
-  if (split < 2) return p;
-  p.tail = static_cast<int>(tail);
-  p.split = static_cast<int>(split);
-  p.bytes = kMxCounterBytes + static_cast<size_t>(tail * split) * 256 * 256 * 4;
+  p.nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int64_t tiles = (N + 127) / 128 * ((M + p.nt - 1) / p.nt), num_kb = (K + kMxStageK - 1) / kMxStageK;
+  // Clusters as long as all CTAs fit at once, two to an SM.
+  while (p.parts < 8 && 2 * p.parts * tiles <= 2 * sms && 2 * p.parts <= num_kb) p.parts *= 2;
   return p;
 }
 
@@ -294,9 +274,9 @@ int usable_sms(const DeviceInfo& d) {
 }
 
 template <int NT, bool F32>
-int launch_few(const MxFewParams& p, const MxPlan& plan, cudaStream_t st) {
-  using Cfg = MxFewCfg<NT, F32>;
-  constexpr auto kern = mx_gemm_few_kernel<Cfg>;
+int launch_cluster(const MxClusterParams& p, const MxPlan& plan, cudaStream_t st) {
+  using Cfg = MxClusterCfg<NT, F32>;
+  constexpr auto kern = mx_gemm_cluster_kernel<Cfg>;
   KernelState& ks = kernel_state<kern>();
   int dev = 0;
   cudaGetDevice(&dev);
@@ -308,24 +288,26 @@ int launch_few(const MxFewParams& p, const MxPlan& plan, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = pair_launch_config(attr, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, st);
   attr[0].val.clusterDim.x = plan.parts;
-  cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * plan.parts));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * p.tiles_x * plan.parts));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "matmul_mxfp4 launch");
 }
 
 template <bool F32>
-int run_few(MxFewParams& p, const MxPlan& plan, cudaStream_t st) {
-  if (p.M <= 16) return launch_few<16, F32>(p, plan, st);
-  if (p.M <= 32) return launch_few<32, F32>(p, plan, st);
-  if (p.M <= 64) return launch_few<64, F32>(p, plan, st);
-  return launch_few<128, F32>(p, plan, st);
+int run_cluster(MxClusterParams& p, const MxPlan& plan, cudaStream_t st) {
+  switch (plan.nt) {
+    case 16: return launch_cluster<16, F32>(p, plan, st);
+    case 32: return launch_cluster<32, F32>(p, plan, st);
+    case 64: return launch_cluster<64, F32>(p, plan, st);
+    default: return launch_cluster<128, F32>(p, plan, st);
+  }
 }
 
 template <bool F32>
 int run_pair(MxParams& p, const DeviceInfo& d, cudaStream_t st) {
   using Cfg = MxCfg<F32>;
-  return launch_pair<mx_gemm_pair_kernel<Cfg>>(p, p.tiles_m * p.tiles_n + p.sk_tail * (p.sk_split - 1),
-                                               Cfg::NUM_THREADS, Cfg::SMEM_BYTES, d, st, "matmul_mxfp4 launch");
+  return launch_pair<mx_gemm_pair_kernel<Cfg>>(p, p.tiles_m * p.tiles_n, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, d, st,
+                                               "matmul_mxfp4 launch");
 }
 
 int check_matmul(int64_t M, int64_t N, int64_t K) {
@@ -340,33 +322,29 @@ int check_matmul(int64_t M, int64_t N, int64_t K) {
 }
 
 int op_matmul(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c, int64_t M, int64_t N,
-              int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+              int64_t K, int out_dtype, cudaStream_t st) {
   if (int rc = check_matmul(M, N, K)) return rc;
   if (int rc = check_dtype(out_dtype)) return rc;
   if (M == 0 || N == 0) return SWIGLU_OK;
   if (!aq || !a_scale || !bq || !b_scale || !c) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
-  if (!aligned16(aq) || !aligned16(a_scale) || !aligned16(bq) || !aligned16(b_scale) || !aligned16(c) ||
-      !aligned16(workspace))
+  if (!aligned16(aq) || !aligned16(a_scale) || !aligned16(bq) || !aligned16(b_scale) || !aligned16(c))
     return fail(SWIGLU_ERR_MISALIGNED, "matmul_mxfp4: pointers must be 16-byte aligned");
   DeviceInfo* d;
   if (int rc = current_device(&d)) return rc;
   const bool f32 = out_dtype == SWIGLU_F32;
   const MxPlan plan = plan_matmul(M, N, K, usable_sms(*d));
-  if (plan.few) {
-    MxFewParams p{};
-    const uint32_t nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  if (!plan.pair) {
+    MxClusterParams p{};
     if (int rc = make_map_bytes(&p.tmW, bq, K / 2, N, K / 2, 128, "B (MXFP4)")) return rc;
-    if (int rc = make_map_bytes(&p.tmX, aq, K / 2, M, K / 2, nt, "A (MXFP4)")) return rc;
+    if (int rc = make_map_bytes(&p.tmX, aq, K / 2, M, K / 2, plan.nt, "A (MXFP4)")) return rc;
     if (int rc = make_map_scales(&p.tmWs, b_scale, N, K, "B scales")) return rc;
     if (int rc = make_map_scales(&p.tmXs, a_scale, M, K, "A scales")) return rc;
     p.out = c;
     p.M = (int)M, p.N = (int)N, p.K = (int)K;
+    p.tiles_x = (int)((M + plan.nt - 1) / plan.nt);
     p.status = d->status;
-    return f32 ? run_few<true>(p, plan, st) : run_few<false>(p, plan, st);
+    return f32 ? run_cluster<true>(p, plan, st) : run_cluster<false>(p, plan, st);
   }
-  if (static_cast<int64_t>(plan.bytes) > workspace_bytes || (plan.bytes && !workspace))
-    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "matmul_mxfp4: workspace of %lld bytes, %lld needed",
-                (long long)workspace_bytes, (long long)plan.bytes);
   MxParams p{};
   if (int rc = make_map_bytes(&p.tmA, aq, K / 2, M, K / 2, 128, "A (MXFP4)")) return rc;
   if (int rc = make_map_bytes(&p.tmB, bq, K / 2, N, K / 2, 128, "B (MXFP4)")) return rc;
@@ -374,16 +352,9 @@ int op_matmul(const void* aq, const void* a_scale, const void* bq, const void* b
   if (int rc = make_map_scales(&p.tmBs, b_scale, N, K, "B scales")) return rc;
   if (int rc = make_store_map(&p.tmC, c, N, M, N, f32)) return rc;
   p.M = (int)M, p.N = (int)N, p.K = (int)K;
-  p.tiles_m = plan.tiles_m, p.tiles_n = plan.tiles_n;
+  p.tiles_m = (int)((M + 255) / 256), p.tiles_n = (int)((N + 255) / 256);
   p.group_m = 16;
   p.status = d->status;
-  p.sk_tail = plan.tail, p.sk_split = plan.split;
-  if (plan.bytes) {
-    p.sk_counters = static_cast<uint32_t*>(workspace);
-    p.sk_partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kMxCounterBytes);
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, kMxCounterBytes, st);
-    if (e != cudaSuccess) return cuda_fail(e, "matmul_mxfp4 workspace");
-  }
   return f32 ? run_pair<true>(p, *d, st) : run_pair<false>(p, *d, st);
 }
 
@@ -404,20 +375,9 @@ int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, in
   return op_dequantize(q, scale, dst, rows, cols, dtype, static_cast<cudaStream_t>(stream));
 }
 
-int swiglu_b200_matmul_mxfp4_workspace(int64_t M, int64_t N, int64_t K, int num_sms, int64_t* bytes) {
-  if (int rc = check_matmul(M, N, K)) return rc;
-  if (!bytes) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
-  if (num_sms < 1) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "num_sms must be positive");
-  const int sms = num_sms - sm_reserve();
-  *bytes = M && N ? static_cast<int64_t>(plan_matmul(M, N, K, sms < 2 ? 2 : sms).bytes) : 0;
-  return SWIGLU_OK;
-}
-
 int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
-                             int64_t M, int64_t N, int64_t K, int out_dtype, void* workspace, int64_t workspace_bytes,
-                             void* stream) {
-  return op_matmul(aq, a_scale, bq, b_scale, c, M, N, K, out_dtype, workspace, workspace_bytes,
-                   static_cast<cudaStream_t>(stream));
+                             int64_t M, int64_t N, int64_t K, int out_dtype, void* stream) {
+  return op_matmul(aq, a_scale, bq, b_scale, c, M, N, K, out_dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

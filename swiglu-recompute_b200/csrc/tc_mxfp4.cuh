@@ -35,10 +35,6 @@ struct MxParams {
   int M, N, K;
   int tiles_m, tiles_n, group_m;
   uint32_t* status;
-  // Split of the last, partial round of tiles along K (see TcParams).
-  float* sk_partials;
-  uint32_t* sk_counters;
-  int sk_tail, sk_split;
 };
 
 // TMEM: two 256-column accumulators that share 120 columns (0..255 and
@@ -141,21 +137,19 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
 
   const int num_kb = (p.K + kMxStageK - 1) / kMxStageK;
   const int tiles = p.tiles_m * p.tiles_n;
-  const int num_units = sk_units(tiles, p.sk_tail, p.sk_split);
-  const int first_unit = static_cast<int>(cluster_id_x());
-  const int unit_step = static_cast<int>(num_clusters_x());
+  const int first_tile = static_cast<int>(cluster_id_x());
+  const int tile_step = static_cast<int>(num_clusters_x());
   uint32_t* status = p.status;
 
   if (warp == 0) {
     uint32_t stage = 0, phase = 0, filled = 0, fill_parity = 0;
     bool ok = true;
-    for (int u = first_unit; u < num_units && ok; u += unit_step) {
-      const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+    for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
       int pm, pn;
-      tile_coords(w.tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
+      tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
       const int am = 2 * pm + static_cast<int>(rank);  // 128-row blocks of A and B of this CTA
       const int bn = 2 * pn + static_cast<int>(rank);
-      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+      for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) {
           ok = false;
           break;
@@ -193,14 +187,13 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
       const uint32_t smem0 = smem_u32(smem);
       uint32_t stage = 0, phase = 0, acc = 0, free_phase = 1;
       bool ok = true;
-      for (int u = first_unit; u < num_units && ok; u += unit_step) {
-        const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
+      for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
         // The previous tile's epilogue has read the columns both accumulators
         // share (and, before that, all of the tile before it).
         if (!mbar_wait_warp(tmem_free, free_phase, abort_flag, status, kErrTimeoutMma)) break;
         free_phase ^= 1;
         const uint32_t d_tmem = tmem_base + acc * Cfg::ACC_STEP;
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_warp(&scaled[stage], phase, abort_flag, status, kErrTimeoutMma)) {
             ok = false;
             break;
@@ -214,10 +207,10 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
             for (int k = 0; k < 4; ++k) {
               umma_mxf4_ss_pair(d_tmem, make_smem_desc_sw128(sa + k * 32, 16, 1024),
                                 make_smem_desc_sw128(sb + k * 32, 16, 1024), idesc[k & 1], sfa + 4 * (k >> 1),
-                                sfb + 8 * (k >> 1), (kb != w.kb0 || k != 0) ? 1u : 0u);
+                                sfb + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
             }
             umma_commit_pair_both(&empty[stage]);
-            if (kb + 1 == w.kb1) umma_commit_pair_both(&tmem_full[acc]);
+            if (kb + 1 == num_kb) umma_commit_pair_both(&tmem_full[acc]);
           }
           __syncwarp();
           if (++stage == STAGES) {
@@ -239,9 +232,8 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
       const uint32_t smem0 = smem_u32(smem);
       uint32_t stage = 0, phase = 0;
       bool ok = true;
-      for (int u = first_unit; u < num_units && ok; u += unit_step) {
-        const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+      for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
+        for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait_warp(&full[stage], phase, abort_flag, status, kErrTimeoutMma)) {
             ok = false;
             break;
@@ -278,54 +270,33 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
     uint32_t acc = 0, acc_phase = 0;
     uint8_t* stage = smem + Cfg::EPI_OFFSET + (warp - 2) * StoreStage<Cfg::OUT_F32>::kWarpBytes;
     constexpr int kBufBytes = StoreStage<Cfg::OUT_F32>::kWarpBytes / 2;
-    auto free_acc = [&] {
+    for (int tile = first_tile; tile < tiles; tile += tile_step) {
+      int pm, pn;
+      tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
+      if (!mbar_wait(&tmem_full[acc], acc_phase, abort_flag, status, kErrTimeoutEpilogue)) break;
+      tc_fence_after_sync();
+      const int row0 = pm * 256 + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
+      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * Cfg::ACC_STEP;
+      // Shared columns first: chunks 7..4 of accumulator 0, 0..3 of accumulator 1.
+      const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
+      uint32_t r[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + i * c_step) * 32, r[i]);
+      tmem_ld_wait();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(map_to_rank(tmem_free, 0));
-    };
-    for (int u = first_unit; u < num_units; u += unit_step) {
-      const SkUnit w = sk_unit_of(tiles, p.sk_tail, p.sk_split, u, num_kb);
-      int pm, pn;
-      tile_coords(w.tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
-      if (!mbar_wait(&tmem_full[acc], acc_phase, abort_flag, status, kErrTimeoutEpilogue)) break;
-      tc_fence_after_sync();
-      const int row_in_tile = 128 * static_cast<int>(rank) + static_cast<int>(q * 32 + lane);
-      const int row0 = pm * 256 + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
-      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * Cfg::ACC_STEP;
-      bool mine = true, freed = false;
-      if (w.parts > 1) {
-        // A part of a split tile: the last to arrive for this 32-row slab
-        // finishes it. The sum is built in TMEM, so nothing is freed early.
-        const int i = w.tile - (tiles - p.sk_tail);
-        const long long part_stride = 256ll * 256;
-        const float* fix = p.sk_partials + (static_cast<long long>(i) * w.parts * 256 + row_in_tile) * 256;
-        mine = sk_publish_and_fix(t_row, 256, const_cast<float*>(fix) + w.part * part_stride, fix, part_stride,
-                                  w.parts, p.sk_counters + i * 8 + rank * 4 + q, 1);
-      }
-      if (mine) {
-        // Shared columns first: chunks 7..4 of accumulator 0, 0..3 of accumulator 1.
-        const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
-        uint32_t r[4][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + i * c_step) * 32, r[i]);
-        tmem_ld_wait();
-        if (w.parts == 1) {
-          free_acc();
-          freed = true;
-        }
+      for (int i = 0; i < 4; ++i)
+        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
+                                     pn * 256 + (c_first + i * c_step) * 32, row0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
-                                       pn * 256 + (c_first + i * c_step) * 32, row0);
+      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + (4 + i) * c_step) * 32, r[i]);
+      tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + (4 + i) * c_step) * 32, r[i]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
-                                       pn * 256 + (c_first + (4 + i) * c_step) * 32, row0);
-      }
-      if (!freed) free_acc();
+      for (int i = 0; i < 4; ++i)
+        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
+                                     pn * 256 + (c_first + (4 + i) * c_step) * 32, row0);
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
@@ -343,23 +314,26 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
   }
 }
 
-// ------------------------------------------------------------ few rows
-// M <= 128: the roles are swapped. The tensor core's 128-row operand is a tile
-// of B (the weight), its columns are the M tokens padded to NT, so a weight
-// byte is loaded once and no part of a tile is wasted on rows that do not
-// exist. The work is the weight's bytes; when its tiles are fewer than the
-// CTAs that fit, a cluster of CTAs shares a tile and splits K, and the parts
-// are added in rank order through distributed shared memory.
-struct MxFewParams {
+// ------------------------------------------------------------ clusters along K
+// The kernel for outputs with too few 256 x 256 tiles to fill the device. The
+// roles are swapped: the tensor core's 128-row operand is a tile of B (the
+// weight), its columns are NT of A's M rows (the tokens; NT = 16..128), so with
+// one token a weight byte is loaded once and nothing is padded but the columns.
+// While the tiles are fewer than the CTAs that fit, a cluster of up to eight
+// CTAs shares a tile and splits K; the parts are added in rank order through
+// distributed shared memory, so no workspace is needed and results are
+// run-to-run identical.
+struct MxClusterParams {
   CUtensorMap tmW, tmWs;  // weight codes {128 bytes, 128 rows}, its scale tiles
   CUtensorMap tmX, tmXs;  // token codes {128 bytes, NT rows}, their scale tiles
   void* out;              // [M, N]
   int M, N, K;
+  int tiles_x;            // token tiles
   uint32_t* status;
 };
 
 template <int NT_, bool OUT_F32_>
-struct MxFewCfg {
+struct MxClusterCfg {
   static constexpr int NT = NT_;
   static constexpr bool OUT_F32 = OUT_F32_;
   static constexpr int W_BYTES = 128 * 128;
@@ -385,7 +359,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 }
 
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __grid_constant__ MxFewParams p) {
+__global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_cluster_kernel(const __grid_constant__ MxClusterParams p) {
   constexpr int STAGES = Cfg::STAGES, NT = Cfg::NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -398,7 +372,10 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
   const uint32_t warp = warp_id(), lane = lane_id();
   const int rank = static_cast<int>(cluster_ctarank());
   const int parts = static_cast<int>(gridDim.x) / static_cast<int>(num_clusters_x());  // cluster size
-  const int tile = static_cast<int>(cluster_id_x());
+  // Token tiles innermost: neighbours read the same weight tile.
+  const int cluster = static_cast<int>(cluster_id_x());
+  const int tile = cluster / p.tiles_x, x_tile = cluster % p.tiles_x;
+  const int x0 = x_tile * NT, tokens = min(NT, p.M - x0);
   const int num_kb = (p.K + kMxStageK - 1) / kMxStageK;
   const int kb0 = rank * num_kb / parts, kb1 = (rank + 1) * num_kb / parts;
 
@@ -430,8 +407,8 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
         mbar_arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
         tma_load_2d(s, &p.tmW, &full[stage], kb * 128, tile * 128);
         tma_load_2d(s + Cfg::SFW_OFFSET, &p.tmWs, &full[stage], kb * 256, tile);
-        tma_load_2d(s + Cfg::W_BYTES, &p.tmX, &full[stage], kb * 128, 0);
-        tma_load_2d(s + Cfg::SFX_OFFSET, &p.tmXs, &full[stage], kb * 256, 0);
+        tma_load_2d(s + Cfg::W_BYTES, &p.tmX, &full[stage], kb * 128, x0);
+        tma_load_2d(s + Cfg::SFX_OFFSET, &p.tmXs, &full[stage], kb * 256, x0 / 128);
       }
       __syncwarp();
       filled |= 1u << stage;
@@ -492,7 +469,7 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
 
   // Output of one token and weight row.
   auto store = [&](int token, int row, float v) {
-    const long long at = static_cast<long long>(token) * p.N + tile * 128ll + row;
+    const long long at = static_cast<long long>(x0 + token) * p.N + tile * 128ll + row;
     if (tile * 128 + row < p.N) {
       if constexpr (Cfg::OUT_F32) static_cast<float*>(p.out)[at] = v;
       else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
@@ -508,13 +485,13 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
       const uint32_t t_row = tmem_base + (((warp & 3u) * 32u) << 16);
 #pragma unroll
       for (int c = 0; c < NT; c += 16) {
-        if (c >= p.M) break;
+        if (c >= tokens) break;
         uint32_t r[16];
         tmem_ld_32x32b_x16(t_row + c, r);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (c + i < p.M) {
+          if (c + i < tokens) {
             if (parts == 1) store(c + i, row, __uint_as_float(r[i]));
             else part[(c + i) * 128 + row] = __uint_as_float(r[i]);
           }
@@ -525,10 +502,14 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_few_kernel(const __g
   if (parts > 1) {
     cluster_sync_all();
     if (warp >= 2 && ok) {
-      for (int t = rank; t < p.M; t += parts) {
-        float v = 0.0f;
-        for (int s = 0; s < parts; ++s) v += ld_cluster_f32(map_to_rank(&part[t * 128 + row], s));
-        store(t, row, v);
+#pragma unroll 2
+      for (int t = rank; t < tokens; t += parts) {
+        float v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v[s] = s < parts ? ld_cluster_f32(map_to_rank(&part[t * 128 + row], s)) : 0.0f;
+#pragma unroll
+        for (int s = 1; s < 8; ++s) v[0] += v[s];
+        store(t, row, v[0]);
       }
     }
     cluster_sync_all();  // no CTA leaves while another reads its parts

@@ -62,8 +62,7 @@ _SIGNATURES = {
     "swiglu_b200_clip_grads_by_norm": [_p, _p, _p, _p, _i64, _p, _p, _p],
     "swiglu_b200_quantize_mxfp4": [_p, _p, _p, _i64, _i64, _i, _p],
     "swiglu_b200_dequantize_mxfp4": [_p, _p, _p, _i64, _i64, _i, _p],
-    "swiglu_b200_matmul_mxfp4_workspace": [_i64, _i64, _i64, _i, ctypes.POINTER(_i64)],
-    "swiglu_b200_matmul_mxfp4": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _i64, _p],
+    "swiglu_b200_matmul_mxfp4": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p],
     "swiglu_b200_mlp_forward":
         [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _p],
     "swiglu_b200_mlp_backward":

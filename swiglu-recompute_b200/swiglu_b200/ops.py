@@ -509,10 +509,6 @@ def mxfp4_scale_shape(rows: int, cols: int) -> tuple[int, int, int, int, int]:
     return (-(-rows // 128), -(-cols // 128), 32, 4, 4)
 
 
-# Rows up to which the product runs without a workspace (kFewRows of mxfp4.cu).
-_MXFP4_FEW_ROWS = 128
-
-
 def _check_mx(q: torch.Tensor, scale: torch.Tensor) -> tuple[int, int]:
     if q.dtype != torch.uint8 or scale.dtype != torch.uint8 or q.dim() != 2:
         raise TypeError("an MXFP4 matrix is a uint8 [R, K / 2] tensor of codes and a uint8 tensor of scales")
@@ -559,12 +555,6 @@ def matmul_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_sc
     if K != K2:
         raise ValueError(f"inner dimensions differ: {K} vs {K2}")
     out = torch.empty((M, N), device=dev, dtype=out_dtype)
-    odt = dtype_code(out_dtype)
-    ws, size = None, ctypes.c_int64(0)
-    if M > _MXFP4_FEW_ROWS:  # fewer rows never need a workspace
-        _lib.call("swiglu_b200_matmul_mxfp4_workspace", M, N, K, _num_sms(dev), ctypes.byref(size))
-        if size.value:
-            ws = torch.empty((size.value,), device=dev, dtype=torch.uint8)
     _launch(dev, "swiglu_b200_matmul_mxfp4", aq.data_ptr(), a_scale.data_ptr(), bq.data_ptr(), b_scale.data_ptr(),
-            out.data_ptr(), M, N, K, odt, _ptr(ws), size.value)
+            out.data_ptr(), M, N, K, dtype_code(out_dtype))
     return out
