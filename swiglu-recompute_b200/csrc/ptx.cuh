@@ -254,11 +254,12 @@ __device__ __forceinline__ uint32_t num_clusters_x() {
 }
 
 // Shared::cluster address of the same variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t rank) {
   uint32_t out;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_addr), "r"(rank));
   return out;
 }
+__device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) { return map_to_rank(smem_u32(p), rank); }
 
 // Arrive on an mbarrier given by shared::cluster address (possibly the
 // peer's), with the instruction's default (.release, .cta) semantics. Callers

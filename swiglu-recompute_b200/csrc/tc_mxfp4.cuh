@@ -341,8 +341,8 @@ struct MxClusterCfg {
   static constexpr int SFW_OFFSET = W_BYTES + X_BYTES;
   static constexpr int SFX_OFFSET = SFW_OFFSET + kMxScaleBytes;
   static constexpr int STAGE_BYTES = SFX_OFFSET + kMxScaleBytes;
-  // About 100 KB a CTA, two CTAs an SM: twice what the latency of HBM asks for.
-  static constexpr int STAGES = 100 * 1024 / STAGE_BYTES;
+  // About 105 KB a CTA, two CTAs an SM: twice what the latency of HBM asks for.
+  static constexpr int STAGES = 107 * 1024 / STAGE_BYTES;
   static constexpr int SF_COL = NT;  // scale buffers: 16 columns each
   static constexpr int TMEM_COLS = NT + 32 <= 64 ? 64 : NT + 32 <= 128 ? 128 : 256;
   static constexpr int NUM_THREADS = 192;
@@ -352,9 +352,12 @@ struct MxClusterCfg {
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -467,53 +470,53 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_cluster_kernel(const
     mbar_wait_warp(tmem_full, 0, &never, status, kErrTimeoutTeardown);
   }
 
-  // Output of one token and weight row.
-  auto store = [&](int token, int row, float v) {
-    const long long at = static_cast<long long>(x0 + token) * p.N + tile * 128ll + row;
-    if (tile * 128 + row < p.N) {
-      if constexpr (Cfg::OUT_F32) static_cast<float*>(p.out)[at] = v;
-      else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    }
-  };
-  const int row = static_cast<int>((warp & 3u) * 32 + lane);  // TMEM lane = weight row (warps 2..5)
-  float* part = reinterpret_cast<float*>(smem);               // [NT][128], over the ring once its MMAs are done
+  // Each CTA lays its part down as [token][weight row] over the ring (its MMAs
+  // are done), then the CTAs of the cluster share the tokens: a thread adds four
+  // neighbouring rows of a token over the parts, in rank order, and stores them.
+  float* part = reinterpret_cast<float*>(smem);
   bool ok = true;
   if (warp >= 2) {
     ok = mbar_wait(tmem_full, 0, abort_flag, status, kErrTimeoutEpilogue);
     if (ok) {
       tc_fence_after_sync();
-      const uint32_t t_row = tmem_base + (((warp & 3u) * 32u) << 16);
-#pragma unroll
-      for (int c = 0; c < NT; c += 16) {
-        if (c >= tokens) break;
+      const uint32_t q = warp & 3u;
+      const int row = static_cast<int>(q * 32 + lane);  // TMEM lane = weight row
+#pragma unroll 1
+      for (int c = 0; c < tokens; c += 16) {
         uint32_t r[16];
-        tmem_ld_32x32b_x16(t_row + c, r);
+        tmem_ld_32x32b_x16(tmem_base + ((q * 32u) << 16) + c, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (c + i < tokens) {
-            if (parts == 1) store(c + i, row, __uint_as_float(r[i]));
-            else part[(c + i) * 128 + row] = __uint_as_float(r[i]);
-          }
-        }
+        for (int i = 0; i < 16; ++i) part[(c + i) * 128 + row] = __uint_as_float(r[i]);
       }
     }
   }
-  if (parts > 1) {
-    cluster_sync_all();
-    if (warp >= 2 && ok) {
-#pragma unroll 2
-      for (int t = rank; t < tokens; t += parts) {
-        float v[8];
+  if (parts > 1) cluster_sync_all();
+  else if (warp >= 2) asm volatile("bar.sync 1, 128;" ::: "memory");
+  const int n = tile * 128 + static_cast<int>(lane) * 4;
+  if (warp >= 2 && ok && n < p.N) {  // N is a multiple of 8: groups of four are whole
+    const uint32_t mine = smem_u32(part) + lane * 16;
+#pragma unroll 4
+    for (int t = rank + static_cast<int>(warp - 2) * parts; t < tokens; t += 4 * parts) {
+      float4 v[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) v[s] = s < parts ? ld_cluster_f32(map_to_rank(&part[t * 128 + row], s)) : 0.0f;
+      for (int s = 0; s < 8; ++s) {
+        if (s < parts) v[s] = ld_cluster_f32x4(map_to_rank(mine + t * 512, s));
+      }
 #pragma unroll
-        for (int s = 1; s < 8; ++s) v[0] += v[s];
-        store(t, row, v[0]);
+      for (int s = 1; s < 8; ++s) {
+        if (s < parts) v[0] = make_float4(v[0].x + v[s].x, v[0].y + v[s].y, v[0].z + v[s].z, v[0].w + v[s].w);
+      }
+      const long long at = static_cast<long long>(x0 + t) * p.N + n;
+      if constexpr (Cfg::OUT_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v[0];
+      } else {
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+            make_uint2(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[0].z, v[0].w));
       }
     }
-    cluster_sync_all();  // no CTA leaves while another reads its parts
   }
+  if (parts > 1) cluster_sync_all();  // no CTA leaves while another reads its part
 
   tc_fence_before_sync();
   __syncthreads();
