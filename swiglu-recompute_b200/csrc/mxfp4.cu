@@ -255,17 +255,45 @@ struct MxPlan {
   int nt, parts;
 };
 
+// Times in us, fitted to measurements of every form on one B200 (148 SMs) over
+// 40 shapes (M 1..4096, N 128..28672, K 512..28672), most within 15 %:
+//   pair     5.2 + rounds * (0.37 a k-block + 1)
+//   cluster  per wave of two CTAs an SM, start and end, 0.35..0.43 a k-block of
+//            a CTA (half as much again while two share an SM), and the join
+// e.g. 256 x 3584 x 3584: pair 10.6, 128 columns on one CTA 12.6, on two 10.6;
+// 333 x 1000 x 14336: pair 24.3, 128 on one 29.2, on four 12.6, on eight 12.4;
+// 1024 x 3584 x 3584: pair 11.0, 128 on one 15.3; 1 x 3584 x 14336: 16 columns
+// on one CTA 23.0, on two 14.3, on four 10.1, on eight 9.5.
 MxPlan plan_matmul(int64_t M, int64_t N, int64_t K, int sms) {
-  MxPlan p{false, 128, 1};
-  if (M > 128 && (M + 255) / 256 * ((N + 255) / 256) >= sms / 2) {
-    p.pair = true;
-    return p;
+  struct Width {
+    int nt;
+    float start, block, join[4];  // join: 1, 2, 4, 8 CTAs
+  };
+  constexpr Width kWidths[] = {{16, 3.3f, 0.345f, {0.0f, 0.7f, 1.2f, 2.2f}},
+                               {32, 3.6f, 0.355f, {0.0f, 1.0f, 1.6f, 3.0f}},
+                               {64, 4.4f, 0.36f, {0.0f, 1.5f, 2.4f, 4.4f}},
+                               {128, 6.0f, 0.43f, {0.0f, 1.5f, 2.4f, 4.4f}}};
+  const int64_t num_kb = (K + kMxStageK - 1) / kMxStageK, tiles_w = (N + 127) / 128;
+  MxPlan best{true, 256, 1};
+  const int64_t pairs = sms / 2;
+  const int64_t rounds = ((M + 255) / 256 * ((N + 255) / 256) + pairs - 1) / pairs;
+  float best_us = 4.2f + static_cast<float>(rounds) * (0.37f * static_cast<float>(num_kb) + 1.0f);
+  if (M <= 64) best_us = 1e30f;  // three quarters of a pair tile would be padding
+  for (const Width& w : kWidths) {
+    // A narrow tile holds all rows: a second one would start inside a scale tile.
+    if (w.nt < 128 && M > w.nt) continue;
+    const int64_t tiles = tiles_w * ((M + w.nt - 1) / w.nt);
+    for (int i = 0, parts = 1; i < 4 && parts <= num_kb; ++i, parts *= 2) {
+      const int64_t ctas = tiles * parts, waves = (ctas + 2 * sms - 1) / (2 * sms);
+      const float blocks = static_cast<float>((num_kb + parts - 1) / parts) * (ctas > sms ? 1.5f : 1.0f);
+      const float us = static_cast<float>(waves) * (w.start + w.block * blocks + w.join[i]);
+      if (us < best_us) {
+        best_us = us;
+        best = MxPlan{false, w.nt, parts};
+      }
+    }
   }
-  p.nt = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const int64_t tiles = (N + 127) / 128 * ((M + p.nt - 1) / p.nt), num_kb = (K + kMxStageK - 1) / kMxStageK;
-  // Clusters as long as all CTAs fit at once, two to an SM.
-  while (p.parts < 8 && 2 * p.parts * tiles <= 2 * sms && 2 * p.parts <= num_kb) p.parts *= 2;
-  return p;
+  return best;
 }
 
 int usable_sms(const DeviceInfo& d) {
