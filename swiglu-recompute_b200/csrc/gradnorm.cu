@@ -22,6 +22,7 @@ namespace {
 constexpr int kTableTensors = 112;  // one launch's table stays below 4 KB of parameters
 constexpr int kGradThreads = 256;
 constexpr int kGradSlots = 8;       // 16-byte slots per thread and chunk
+constexpr int kGradBlocks = 4;      // per SM
 constexpr int kChunkSlots = kGradThreads * kGradSlots;
 
 struct GradTable {
@@ -50,31 +51,58 @@ __device__ __forceinline__ int tensor_of(const GradTable& t, int chunk) {
   return lo;
 }
 
-// The elements of slot `v` of a tensor that starts `head` elements after a
-// 16-byte boundary: f[e] for the N elements, zero outside the tensor.
+// A thread's slots of one chunk of tensor k. Slots wholly inside the tensor are
+// 16-byte words; in the others, at its ends, elements outside are zeros.
 template <typename T>
-struct Slot {
+struct ChunkSlots {
   static constexpr int N = 16 / sizeof(T);
-  __device__ static void load(const T* base, long long e0, long long size, float (&f)[N]) {
-    if (e0 >= 0 && e0 + N <= size) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(base + e0));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  const T* base;
+  long long size, e0;  // the tensor's elements; the first element of this thread's first slot
+  bool whole;          // all slots of the chunk (any thread's) are inside
+
+  __device__ __forceinline__ ChunkSlots(const GradTable& t, int k, int chunk) {
+    base = static_cast<const T*>(t.in[k]);
+    size = t.size[k];
+    const int head = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 16 / sizeof(T));
+    const long long c0 = static_cast<long long>(chunk - t.first_chunk[k]) * (kChunkSlots * N) - head;
+    whole = c0 >= 0 && c0 + kChunkSlots * N <= size;
+    e0 = c0 + static_cast<long long>(threadIdx.x) * N;
+  }
+  __device__ __forceinline__ long long at(int i) const { return e0 + i * (kGradThreads * N); }
+  __device__ __forceinline__ bool inside(int i) const { return at(i) >= 0 && at(i) + N <= size; }
+  __device__ __forceinline__ void load(uint4 (&u)[kGradSlots]) const {
+    if (whole) {
+      const uint4* p = reinterpret_cast<const uint4*>(base + e0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          f[i] = __uint_as_float(w[i]);
-        } else {
-          const float2 v = unpack_bf16x2(w[i]);
-          f[2 * i] = v.x;
-          f[2 * i + 1] = v.y;
-        }
-      }
+      for (int i = 0; i < kGradSlots; ++i) u[i] = __ldg(p + i * kGradThreads);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const bool in = e0 + i >= 0 && e0 + i < size;
-        if constexpr (sizeof(T) == 4) f[i] = in ? base[e0 + i] : 0.0f;
-        else f[i] = in ? __bfloat162float(base[e0 + i]) : 0.0f;
+      for (int i = 0; i < kGradSlots; ++i) {
+        if (inside(i)) {
+          u[i] = __ldg(reinterpret_cast<const uint4*>(base + at(i)));
+        } else {
+          uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            if (at(i) + e < 0 || at(i) + e >= size) continue;
+            if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(base[at(i) + e]);
+            else w[e / 2] |= static_cast<uint32_t>(__bfloat16_as_ushort(base[at(i) + e])) << (16 * (e & 1));
+          }
+          u[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+  __device__ static __forceinline__ void values(const uint4& u, float (&f)[N]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        const float2 v = unpack_bf16x2(w[i]);
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
       }
     }
   }
@@ -82,26 +110,26 @@ struct Slot {
 
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const GradTable& t, int k, int chunk) {
-  constexpr int N = Slot<T>::N;
-  const T* base = static_cast<const T*>(t.in[k]);
-  const long long size = t.size[k];
-  const int head = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 16 / sizeof(T));
-  const long long v0 = static_cast<long long>(chunk - t.first_chunk[k]) * kChunkSlots + threadIdx.x;
-  float f[kGradSlots][N];
-#pragma unroll
-  for (int i = 0; i < kGradSlots; ++i) Slot<T>::load(base, (v0 + i * kGradThreads) * N - head, size, f[i]);
-  float sum = 0.0f;
+  constexpr int N = ChunkSlots<T>::N;
+  uint4 u[kGradSlots];
+  ChunkSlots<T>(t, k, chunk).load(u);
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kGradSlots; ++i) {
+    float f[N];
+    ChunkSlots<T>::values(u[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum += f[i][e] * f[i][e];
+    for (int e = 0; e < N; ++e) sum[e & 3] += f[e] * f[e];
   }
-  if (sum >= 1e-30f && sum <= 1e37f) return static_cast<double>(sum);
+  const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  if (total >= 1e-30f && total <= 1e37f) return static_cast<double>(total);
   double exact = 0.0;
-#pragma unroll 1
-  for (int i = 0; i < kGradSlots; ++i) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) exact += static_cast<double>(f[i][e]) * static_cast<double>(f[i][e]);
+  for (int i = 0; i < kGradSlots; ++i) {
+    float f[N];
+    ChunkSlots<T>::values(u[i], f);
+#pragma unroll
+    for (int e = 0; e < N; ++e) exact += static_cast<double>(f[e]) * static_cast<double>(f[e]);
   }
   return exact;
 }
@@ -118,11 +146,13 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kGradThreads) grad_squares_kernel(const __grid_constant__ GradTable t,
-                                                                    double* partial) {
+__global__ void __launch_bounds__(kGradThreads, kGradBlocks)
+    grad_squares_kernel(const __grid_constant__ GradTable t, double* partial) {
   double sum = 0.0;
-  for (int c = blockIdx.x; c < t.first_chunk[t.count]; c += gridDim.x) {
-    const int k = tensor_of(t, c);
+  const int chunks = t.first_chunk[t.count];
+  int k = blockIdx.x < chunks ? tensor_of(t, blockIdx.x) : 0;
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    while (c >= t.first_chunk[k + 1]) ++k;
     sum += t.f32[k] ? chunk_squares<float>(t, k, c) : chunk_squares<__nv_bfloat16>(t, k, c);
   }
   sum = block_sum(sum);
@@ -142,37 +172,34 @@ __global__ void __launch_bounds__(kGradThreads) grad_norm_kernel(const double* p
 
 template <typename T>
 __device__ __forceinline__ void chunk_scale(const GradTable& t, int k, int chunk, float factor) {
-  constexpr int N = Slot<T>::N;
-  const T* base = static_cast<const T*>(t.in[k]);
+  constexpr int N = ChunkSlots<T>::N;
+  const ChunkSlots<T> slots(t, k, chunk);
   T* out = static_cast<T*>(t.out[k]);
-  const long long size = t.size[k];
-  const int head = static_cast<int>(reinterpret_cast<uintptr_t>(base) % 16 / sizeof(T));
-  const bool same = (reinterpret_cast<uintptr_t>(base) ^ reinterpret_cast<uintptr_t>(out)) % 16 == 0;
-  const long long v0 = static_cast<long long>(chunk - t.first_chunk[k]) * kChunkSlots + threadIdx.x;
-  float f[kGradSlots][N];
-#pragma unroll
-  for (int i = 0; i < kGradSlots; ++i) Slot<T>::load(base, (v0 + i * kGradThreads) * N - head, size, f[i]);
+  const bool same = (reinterpret_cast<uintptr_t>(slots.base) ^ reinterpret_cast<uintptr_t>(out)) % 16 == 0;
+  uint4 u[kGradSlots];
+  slots.load(u);
 #pragma unroll
   for (int i = 0; i < kGradSlots; ++i) {
-    const long long e0 = (v0 + i * kGradThreads) * N - head;
+    float f[N];
+    ChunkSlots<T>::values(u[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[i][e] *= factor;
-    if (same && e0 >= 0 && e0 + N <= size) {
-      uint4 u;
+    for (int e = 0; e < N; ++e) f[e] *= factor;
+    const long long at = slots.at(i);
+    if (same && (slots.whole || slots.inside(i))) {
+      uint4 r;
       if constexpr (sizeof(T) == 4) {
-        u = make_uint4(__float_as_uint(f[i][0]), __float_as_uint(f[i][1]), __float_as_uint(f[i][2]),
-                       __float_as_uint(f[i][3]));
+        r = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
       } else {
-        u = make_uint4(pack_bf16x2(f[i][0], f[i][1]), pack_bf16x2(f[i][2], f[i][3]),
-                       pack_bf16x2(f[i][4], f[i][5]), pack_bf16x2(f[i][6], f[i][7]));
+        r = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                       pack_bf16x2(f[6], f[7]));
       }
-      *reinterpret_cast<uint4*>(out + e0) = u;
+      *reinterpret_cast<uint4*>(out + at) = r;
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        if (e0 + e >= 0 && e0 + e < size) {
-          if constexpr (sizeof(T) == 4) out[e0 + e] = f[i][e];
-          else out[e0 + e] = __float2bfloat16_rn(f[i][e]);
+        if (at + e >= 0 && at + e < slots.size) {
+          if constexpr (sizeof(T) == 4) out[at + e] = f[e];
+          else out[at + e] = __float2bfloat16_rn(f[e]);
         }
       }
     }
@@ -183,26 +210,27 @@ __device__ __forceinline__ void chunk_scale(const GradTable& t, int k, int chunk
 // block adds them up for itself; the first writes it to norm_out) or, with
 // count == 0, from *norm_in. Chunks are walked from the last to the first: the
 // squares pass ended there, so that part is still in L2.
-__global__ void __launch_bounds__(kGradThreads) grad_scale_kernel(const __grid_constant__ GradTable t,
-                                                                  const double* partial, int count,
-                                                                  const float* norm_in, float* norm_out,
-                                                                  double max_norm) {
+__global__ void __launch_bounds__(kGradThreads, kGradBlocks)
+    grad_scale_kernel(const __grid_constant__ GradTable t, const double* partial, int count, const float* norm_in,
+                      float* norm_out, double max_norm) {
   const double n = count ? total_norm(partial, count) : static_cast<double>(*norm_in);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(n);
   double ratio = max_norm / (n + 1e-6);
   if (ratio > 1.0) ratio = 1.0;  // a NaN norm stays one, and reaches every gradient
   const float factor = static_cast<float>(ratio);
-  const int chunks = t.first_chunk[t.count];
-  for (int c = chunks - 1 - static_cast<int>(blockIdx.x); c >= 0; c -= gridDim.x) {
-    const int k = tensor_of(t, c);
+  const int last = t.first_chunk[t.count] - 1 - static_cast<int>(blockIdx.x);
+  int k = last >= 0 ? tensor_of(t, last) : 0;
+  for (int c = last; c >= 0; c -= gridDim.x) {
+    while (c < t.first_chunk[k]) --k;
     if (factor == 1.0f && t.out[k] == t.in[k]) continue;  // x * 1 in place
     if (t.f32[k]) chunk_scale<float>(t, k, c, factor);
     else chunk_scale<__nv_bfloat16>(t, k, c, factor);
   }
 }
 
+// Blocks of a launch: as many as are resident at once.
 int grad_grid(int chunks, int sms) {
-  const int most = sms * 8;
+  const int most = sms * kGradBlocks;
   return chunks < most ? (chunks < 1 ? 1 : chunks) : most;
 }
 
@@ -383,7 +411,7 @@ extern "C" {
 int swiglu_b200_grad_norm_workspace(int64_t count, int num_sms, int64_t* doubles) {
   if (int rc = check_dims("grad_norm_workspace", count, num_sms, 0)) return rc;
   if (!doubles) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
-  const int64_t n = launches_of(count) * num_sms * 8;
+  const int64_t n = launches_of(count) * num_sms * kGradBlocks;
   *doubles = n > 0 ? n : 1;
   return SWIGLU_OK;
 }

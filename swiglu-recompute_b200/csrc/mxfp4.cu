@@ -29,31 +29,6 @@ constexpr int kTileBytes = kMxTileBytes;
 constexpr int kQuantCols = 256;     // columns of one CTA: a warp covers a row of them, 8 a thread
 constexpr int kQuantThreads = 256;
 
-// Eight consecutive values of a row.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = unpack_bf16x2(w[i]);
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
-}
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-  f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                            pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-}
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-
 __device__ __forceinline__ float power_of_two(int field) { return __uint_as_float(static_cast<uint32_t>(field) << 23); }
 
 // 2^(byte - 127): byte 0 is the subnormal 2^-127, byte 255 a NaN.
@@ -67,57 +42,91 @@ __device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
   return __half22float2(__half2(h));
 }
 
-// One CTA: 128 rows x 256 columns, two scale tiles. A warp reads 256 columns
-// of one row (512 bytes of bf16), eight rows in flight a thread; four lanes
-// share a block, and the tiles' bytes leave together, so that no scale byte is
-// written alone.
+// One CTA: 128 rows x 256 columns, two scale tiles. A warp takes a row at a time,
+// 16 bytes a lane (bf16: all 256 columns, four lanes a block; f32: twice 128,
+// eight lanes a block), several rows in flight; the scale bytes are collected in
+// shared memory and leave as whole tiles, none is written alone.
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) quantize_mxfp4_kernel(const T* __restrict__ src,
-                                                                       uint8_t* __restrict__ dst,
-                                                                       uint8_t* __restrict__ scale, long long rows,
-                                                                       int cols, int tiles_k) {
+struct MxLanes {
+  static constexpr int E = 16 / sizeof(T);             // elements of a lane
+  static constexpr int GROUPS = kQuantCols / (32 * E); // loads that make the 256 columns
+  static constexpr int LANES = kBlock / E;             // lanes that share a block
+  static constexpr int BATCH = 8 / GROUPS;             // rows in flight
+};
+
+// |v| as an integer compares as |v|, and a NaN is above infinity: the exponent
+// field of the largest of a lane's elements.
+template <typename T>
+__device__ __forceinline__ uint32_t top_exponent(const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m >> 23;
+  } else {
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                                __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16) >> 7;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads, 4) quantize_mxfp4_kernel(const T* __restrict__ src,
+                                                                          uint8_t* __restrict__ dst,
+                                                                          uint8_t* __restrict__ scale, long long rows,
+                                                                          int cols, int tiles_k) {
+  using L = MxLanes<T>;
   __shared__ __align__(16) uint8_t tile[2 * kTileBytes];
   const int lane = static_cast<int>(lane_id()), warp = static_cast<int>(warp_id());
-  const long long r0 = blockIdx.y * static_cast<long long>(kTileRows);
-  const int c0 = blockIdx.x * kQuantCols + lane * 8;
-  const bool in_cols = c0 < cols;  // cols is a multiple of 32: whole groups of 8
+  const long long r0 = blockIdx.y * static_cast<long long>(kTileRows) + warp;
+  const int c0 = blockIdx.x * kQuantCols + lane * L::E;
   reinterpret_cast<uint32_t*>(tile)[threadIdx.x] = 0;
   __syncthreads();
+#pragma unroll 1
+  for (int i0 = 0; i0 < 16 && r0 + i0 * 8 < rows; i0 += L::BATCH) {
+    uint4 u[L::BATCH][L::GROUPS];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float f[8][8];
+    for (int i = 0; i < L::BATCH; ++i) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long long r = r0 + (half * 8 + i) * 8 + warp;
-      if (in_cols && r < rows) load8(src + r * cols + c0, f[i]);
+      for (int g = 0; g < L::GROUPS; ++g) {
+        const long long r = r0 + (i0 + i) * 8;
+        const int c = c0 + g * 32 * L::E;
+        u[i][g] = make_uint4(0, 0, 0, 0);
+        if (r < rows && c < cols) u[i][g] = __ldg(reinterpret_cast<const uint4*>(src + r * cols + c));
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int rt = (half * 8 + i) * 8 + warp;
-      const long long r = r0 + rt;
-      const bool in = in_cols && r < rows;
-      uint32_t top = 0;  // |v| compares as an integer; a NaN is above infinity
-      if (in) {
+    for (int i = 0; i < L::BATCH; ++i) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[i][e]) & 0x7fffffffu);
-      }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (!in) continue;
-      const int field = static_cast<int>(top >> 23);  // 127 + floor(log2 max), 0 below the normals
-      const int byte = field == 255 ? 255 : max(field - 2, 0);
-      const float inv = power_of_two(254 - min(byte, 253));
-      uint32_t out = 0;
+      for (int g = 0; g < L::GROUPS; ++g) {
+        const long long r = r0 + (i0 + i) * 8;
+        const int c = c0 + g * 32 * L::E;
+        uint32_t field = top_exponent<T>(u[i][g]);  // 127 + floor(log2 max), 0 below the normals
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __nv_fp4x2_storage_t v = __nv_cvt_float2_to_fp4x2(
-            make_float2(f[i][2 * e] * inv, f[i][2 * e + 1] * inv), __NV_E2M1, cudaRoundNearest);
-        out |= static_cast<uint32_t>(v) << (8 * e);
-      }
-      *reinterpret_cast<uint32_t*>(dst + r * (cols / 2) + c0 / 2) = out;
-      if ((lane & 3) == 0) {
-        const int b = lane >> 2;  // block 0..7 of this CTA's columns
-        tile[(b >> 2) * kTileBytes + (rt & 31) * 16 + (rt >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(byte);
+        for (int o = 1; o < L::LANES; o *= 2) field = max(field, __shfl_xor_sync(0xffffffffu, field, o));
+        if (r >= rows || c >= cols) continue;  // cols is a multiple of 32: a block is inside or not
+        const int byte = field == 255 ? 255 : max(static_cast<int>(field) - 2, 0);
+        const float inv = power_of_two(254 - min(byte, 253));
+        const uint32_t w[4] = {u[i][g].x, u[i][g].y, u[i][g].z, u[i][g].w};
+        uint32_t out = 0;
+#pragma unroll
+        for (int e = 0; e < L::E / 2; ++e) {
+          float2 v;
+          if constexpr (sizeof(T) == 4) v = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+          else v = unpack_bf16x2(w[e]);
+          const __nv_fp4x2_storage_t q =
+              __nv_cvt_float2_to_fp4x2(make_float2(v.x * inv, v.y * inv), __NV_E2M1, cudaRoundNearest);
+          out |= static_cast<uint32_t>(q) << (8 * e);
+        }
+        uint8_t* to = dst + r * (cols / 2) + c / 2;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(out);
+        else *reinterpret_cast<uint32_t*>(to) = out;
+        if (lane % L::LANES == 0) {
+          const int b = (c - static_cast<int>(blockIdx.x) * kQuantCols) / kBlock;  // 0..7 of this CTA's blocks
+          const int rt = (i0 + i) * 8 + warp;
+          tile[(b >> 2) * kTileBytes + (rt & 31) * 16 + (rt >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
@@ -130,43 +139,57 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_mxfp4_kernel(const T* 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) dequantize_mxfp4_kernel(const uint8_t* __restrict__ src,
-                                                                         const uint8_t* __restrict__ scale,
-                                                                         T* __restrict__ dst, long long rows, int cols,
-                                                                         int tiles_k) {
+__global__ void __launch_bounds__(kQuantThreads, 4) dequantize_mxfp4_kernel(const uint8_t* __restrict__ src,
+                                                                            const uint8_t* __restrict__ scale,
+                                                                            T* __restrict__ dst, long long rows,
+                                                                            int cols, int tiles_k) {
+  using L = MxLanes<T>;
   __shared__ __align__(16) uint8_t tile[2 * kTileBytes];
   const int lane = static_cast<int>(lane_id()), warp = static_cast<int>(warp_id());
-  const long long r0 = blockIdx.y * static_cast<long long>(kTileRows);
-  const int c0 = blockIdx.x * kQuantCols + lane * 8;
+  const long long r0 = blockIdx.y * static_cast<long long>(kTileRows) + warp;
+  const int c0 = blockIdx.x * kQuantCols + lane * L::E;
   const int t = 2 * blockIdx.x + (threadIdx.x >> 5);
   if (threadIdx.x < 64 && t < tiles_k) {
     const uint8_t* from = scale + (blockIdx.y * static_cast<long long>(tiles_k) + t) * kTileBytes;
     reinterpret_cast<uint4*>(tile)[threadIdx.x] = __ldg(reinterpret_cast<const uint4*>(from) + (threadIdx.x & 31));
   }
-  const bool in_cols = c0 < cols;
-  uint32_t q[16];
+  uint32_t q[16][L::GROUPS];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const long long r = r0 + i * 8 + warp;
-    if (in_cols && r < rows) q[i] = __ldg(reinterpret_cast<const uint32_t*>(src + r * (cols / 2) + c0 / 2));
+#pragma unroll
+    for (int g = 0; g < L::GROUPS; ++g) {
+      const long long r = r0 + i * 8;
+      const int c = c0 + g * 32 * L::E;
+      if (r < rows && c < cols) {
+        const uint8_t* from = src + r * (cols / 2) + c / 2;
+        if constexpr (sizeof(T) == 4) q[i][g] = __ldg(reinterpret_cast<const uint16_t*>(from));
+        else q[i][g] = __ldg(reinterpret_cast<const uint32_t*>(from));
+      }
+    }
   }
   __syncthreads();
-  if (!in_cols) return;
-  const int b = lane >> 2;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int rt = i * 8 + warp;
-    const long long r = r0 + rt;
-    if (r >= rows) break;
-    const float s = scale_value(tile[(b >> 2) * kTileBytes + (rt & 31) * 16 + (rt >> 5) * 4 + (b & 3)]);
-    float f[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 v = e2m1x2_value((q[i] >> (8 * e)) & 0xffu);
-      f[2 * e] = v.x * s;
-      f[2 * e + 1] = v.y * s;
+    for (int g = 0; g < L::GROUPS; ++g) {
+      const long long r = r0 + i * 8;
+      const int c = c0 + g * 32 * L::E;
+      if (r >= rows || c >= cols) continue;
+      const int b = (c - static_cast<int>(blockIdx.x) * kQuantCols) / kBlock, rt = i * 8 + warp;
+      const float s = scale_value(tile[(b >> 2) * kTileBytes + (rt & 31) * 16 + (rt >> 5) * 4 + (b & 3)]);
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < L::E / 2; ++e) {
+        const float2 v = e2m1x2_value((q[i][g] >> (8 * e)) & 0xffu);
+        if constexpr (sizeof(T) == 4) {
+          w[2 * e] = __float_as_uint(v.x * s);
+          w[2 * e + 1] = __float_as_uint(v.y * s);
+        } else {
+          w[e] = pack_bf16x2(v.x * s, v.y * s);
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + r * cols + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    store8(dst + r * cols + c0, f);
   }
 }
 
