@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 from array import array
+from functools import lru_cache
 
 import torch
 
@@ -334,44 +335,69 @@ def matmul_e4m3(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_sca
 
 
 # ----------------------------------------------------------- helpers of the calls below
+# These calls are also made for single tokens, where the host's time is what a
+# user waits for: outputs come from new_empty (0.5 us less than torch.empty with
+# keywords), checks take one pass, sizes of workspaces are looked up once.
+_CODES = {torch.bfloat16: BF16, torch.float32: F32}
+
+
 def _launch(dev: torch.device, name: str, *args) -> None:
-    """`name(*args, stream)` with `dev` current, on its current torch stream.
-    (Entering the device guard only where another device is current saves about
-    2 us a call, which single-token calls notice.)"""
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch.cuda.current_device() == dev.index:
+    """`name(*args, stream)` with `dev` current, on its current torch stream."""
+    index = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
         _call(dev, name, *args, stream)
     else:
         with torch.cuda.device(dev):
             _call(dev, name, *args, stream)
 
 
-_sms: dict[int, int] = {}
+@lru_cache(maxsize=None)
+def _num_sms(index: int) -> int:
+    return torch.cuda.get_device_properties(index).multi_processor_count
 
 
-def _num_sms(dev: torch.device) -> int:
-    if dev.index not in _sms:
-        _sms[dev.index] = torch.cuda.get_device_properties(dev).multi_processor_count
-    return _sms[dev.index]
+def _query(name: str, *args) -> int:
+    n = ctypes.c_int64(0)
+    _lib.call(name, *args, ctypes.byref(n))
+    return n.value
 
 
-# ------------------------------------------------------------ residual RMS norm
-def _check_norm(x: torch.Tensor, weight: torch.Tensor, *same: torch.Tensor | None) -> tuple[torch.device, int, int]:
-    dev = _check_cuda(x, weight, *same)
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError(f"the norm takes rows [M, D] with D >= 1, got {tuple(x.shape)}")
-    M, D = x.shape
-    if weight.shape != (D,):
-        raise ValueError(f"weight {tuple(weight.shape)} does not match rows of {D}")
-    for t in same:
-        if t is not None and t.shape != x.shape:
-            raise ValueError(f"shapes differ: {tuple(t.shape)} and {tuple(x.shape)}")
-    _same_dtype(x, *same)
-    return dev, M, D
+@lru_cache(maxsize=1024)
+def _rmsnorm_bwd_floats(M: int, D: int, sms: int) -> int:
+    return _query("swiglu_b200_rmsnorm_bwd_workspace", M, D, sms)
+
+
+@lru_cache(maxsize=1024)
+def _grad_norm_doubles(count: int, sms: int) -> int:
+    return _query("swiglu_b200_grad_norm_workspace", count, sms)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+# ------------------------------------------------------------ residual RMS norm
+def _check_norm(x: torch.Tensor, weight: torch.Tensor, *same: torch.Tensor | None):
+    """(device, M, D, dtype codes of x and weight) of a norm's arguments; `same`
+    are the tensors of x's shape and type."""
+    shape, dtype, dev = x.shape, x.dtype, x.device
+    ok = len(shape) == 2 and shape[1] >= 1 and weight.shape == shape[1:]
+    ok = ok and x.is_cuda and x.is_contiguous() and weight.device == dev and weight.is_contiguous()
+    for t in same:
+        if t is not None:
+            ok = ok and t.shape == shape and t.dtype == dtype and t.device == dev and t.is_contiguous()
+    if not ok:
+        _check_cuda(x, weight, *same)
+        if len(shape) != 2 or shape[1] < 1:
+            raise ValueError(f"the norm takes rows [M, D] with D >= 1, got {tuple(shape)}")
+        if weight.shape != shape[1:]:
+            raise ValueError(f"weight {tuple(weight.shape)} does not match rows of {shape[1]}")
+        for t in same:
+            if t is not None and t.shape != shape:
+                raise ValueError(f"shapes differ: {tuple(t.shape)} and {tuple(shape)}")
+        _same_dtype(x, *same)
+    return dev, shape[0], shape[1], dtype_code(dtype), dtype_code(weight.dtype)
 
 
 def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
@@ -379,11 +405,10 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     s = x + residual rounded to x's dtype (x itself without a residual),
     rstd [M] = (mean s^2 + eps)^-1/2 in f32, y = s * rstd * weight in x's dtype.
     weight [D] may be bf16 or f32."""
-    dev, M, D = _check_norm(x, weight, residual)
-    dt, wdt = dtype_code(x.dtype), dtype_code(weight.dtype)
+    dev, M, D, dt, wdt = _check_norm(x, weight, residual)
     y = torch.empty_like(x)
     s = x if residual is None else torch.empty_like(x)
-    rstd = torch.empty((M,), device=dev, dtype=torch.float32)
+    rstd = x.new_empty(M, dtype=torch.float32)
     _launch(dev, "swiglu_b200_rmsnorm_fwd", x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
             s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(eps)), dt, wdt)
     return y, s, rstd
@@ -393,12 +418,11 @@ def rmsnorm_fwd_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
                      eps: float = 1e-6):
     """(q, scale, s, rstd): rmsnorm_fwd with y as row-scaled e4m3 (q [M, D],
     f32 scale [M], as quantize_rows_e4m3 gives them, but from the f32 y)."""
-    dev, M, D = _check_norm(x, weight, residual)
-    dt, wdt = dtype_code(x.dtype), dtype_code(weight.dtype)
-    q = torch.empty((M, D), device=dev, dtype=torch.float8_e4m3fn)
-    scale = torch.empty((M,), device=dev, dtype=torch.float32)
+    dev, M, D, dt, wdt = _check_norm(x, weight, residual)
+    q = x.new_empty((M, D), dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(M, dtype=torch.float32)
     s = x if residual is None else torch.empty_like(x)
-    rstd = torch.empty((M,), device=dev, dtype=torch.float32)
+    rstd = torch.empty_like(scale)
     _launch(dev, "swiglu_b200_rmsnorm_fwd_e4m3", x.data_ptr(), _ptr(residual), weight.data_ptr(), q.data_ptr(),
             scale.data_ptr(), s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(eps)), dt, wdt)
     return q, scale, s, rstd
@@ -409,17 +433,15 @@ def rmsnorm_bwd(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd: t
     """(dx, dweight) of the norm: dx [M, D] is the gradient of x and of the
     residual alike (ds, the gradient of s from its other uses, is added),
     dweight [D] in weight's dtype. s and rstd as the forward returned them."""
-    dev, M, D = _check_norm(s, weight, dy, ds)
+    dev, M, D, dt, wdt = _check_norm(s, weight, dy, ds)
     if rstd.device != dev or rstd.dtype != torch.float32 or rstd.shape != (M,) or not rstd.is_contiguous():
         raise ValueError("rstd must be the forward's f32 [M] tensor")
-    dt, wdt = dtype_code(s.dtype), dtype_code(weight.dtype)
     dx = torch.empty_like(s)
     dweight = torch.empty_like(weight)
-    floats = ctypes.c_int64(0)
-    _lib.call("swiglu_b200_rmsnorm_bwd_workspace", M, D, _num_sms(dev), ctypes.byref(floats))
-    ws = torch.empty((floats.value,), device=dev, dtype=torch.float32)
+    floats = _rmsnorm_bwd_floats(M, D, _num_sms(dev.index))
+    ws = s.new_empty(floats, dtype=torch.float32)
     _launch(dev, "swiglu_b200_rmsnorm_bwd", dy.data_ptr(), s.data_ptr(), weight.data_ptr(), rstd.data_ptr(),
-            _ptr(ds), dx.data_ptr(), dweight.data_ptr(), ws.data_ptr(), floats.value, M, D, dt, wdt)
+            _ptr(ds), dx.data_ptr(), dweight.data_ptr(), ws.data_ptr(), floats, M, D, dt, wdt)
     return dx, dweight
 
 
@@ -428,28 +450,30 @@ class _GradList:
     """Host arrays of a list of gradients, checked."""
 
     def __init__(self, tensors, out=None):
-        self.tensors = list(tensors)
-        if not self.tensors:
+        tensors = self.tensors = list(tensors)
+        if not tensors:
             raise ValueError("no gradients given")
-        dev = self.tensors[0].device
-        for t in self.tensors:
+        dev = self.dev = tensors[0].device
+        for t in tensors:
             if t.device != dev or not t.is_cuda or not t.is_contiguous():
-                _check_cuda(self.tensors[0], t)  # raises with what is wrong
-        self.dev = dev
-        self.dtypes = array("i", [dtype_code(t.dtype) for t in self.tensors])
-        self.sizes = array("q", [t.numel() for t in self.tensors])
-        self.grads = array("Q", [t.data_ptr() for t in self.tensors])
-        self.outs = self.grads
-        self.out = None
+                _check_cuda(tensors[0], t)  # raises with what is wrong
+        try:
+            self.dtypes = array("i", [_CODES[t.dtype] for t in tensors])
+        except KeyError as e:
+            dtype_code(e.args[0])  # raises
+        self.sizes = array("q", [t.numel() for t in tensors])
+        self.grads = array("Q", [t.data_ptr() for t in tensors])
+        self.out, self.outs = tensors, self.grads
         if out is not None:
-            self.out = list(out)
-            if len(self.out) != len(self.tensors):
-                raise ValueError(f"{len(self.out)} outputs for {len(self.tensors)} gradients")
-            for t, o in zip(self.tensors, self.out):
+            out = self.out = list(out)
+            if len(out) != len(tensors):
+                raise ValueError(f"{len(out)} outputs for {len(tensors)} gradients")
+            for t, o in zip(tensors, out):
                 if o.shape != t.shape or o.dtype != t.dtype:
                     raise ValueError("an output differs from its gradient in shape or dtype")
-                _check_cuda(t, o)
-            self.outs = array("Q", [o.data_ptr() for o in self.out])
+                if o.device != dev or not o.is_contiguous():
+                    _check_cuda(t, o)
+            self.outs = array("Q", [o.data_ptr() for o in out])
 
     def args(self, with_outs: bool):
         a = [self.grads.buffer_info()[0]]
@@ -458,19 +482,21 @@ class _GradList:
         return (*a, self.sizes.buffer_info()[0], self.dtypes.buffer_info()[0], len(self.tensors))
 
     def workspace(self) -> torch.Tensor:
-        n = ctypes.c_int64(0)
-        _lib.call("swiglu_b200_grad_norm_workspace", len(self.tensors), _num_sms(self.dev), ctypes.byref(n))
-        return torch.empty((n.value,), device=self.dev, dtype=torch.float64)
+        doubles = _grad_norm_doubles(len(self.tensors), _num_sms(self.dev.index))
+        return self.tensors[0].new_empty(doubles, dtype=torch.float64)
+
+    def norm(self) -> torch.Tensor:
+        return self.tensors[0].new_empty((), dtype=torch.float32)
 
     def written(self) -> None:
-        torch.autograd.graph.increment_version(self.tensors if self.out is None else self.out)
+        torch.autograd.graph.increment_version(self.out)
 
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm (f32, a 0-dim tensor on their device) of all the values of a
     list of contiguous bf16 / f32 tensors on one device."""
     g = _GradList(tensors)
-    norm = torch.empty((), device=g.dev, dtype=torch.float32)
+    norm = g.norm()
     ws = g.workspace()
     _launch(g.dev, "swiglu_b200_grad_norm", *g.args(False), ws.data_ptr(), ws.numel(), norm.data_ptr())
     return norm
@@ -482,10 +508,10 @@ def clip_grad_norm_(tensors, max_norm: float, *, out=None) -> torch.Tensor:
     nothing here waits for it). In place, or into the tensors `out`. A tensor
     that is written may not share memory with another one of the call."""
     g = _GradList(tensors, out)
-    norm = torch.empty((), device=g.dev, dtype=torch.float32)
+    norm = g.norm()
     ws = g.workspace()
-    _launch(g.dev, "swiglu_b200_clip_grad_norm", *g.args(True), ctypes.byref(ctypes.c_double(max_norm)), ws.data_ptr(), ws.numel(),
-            norm.data_ptr())
+    _launch(g.dev, "swiglu_b200_clip_grad_norm", *g.args(True), ctypes.byref(ctypes.c_double(max_norm)),
+            ws.data_ptr(), ws.numel(), norm.data_ptr())
     g.written()
     return norm
 
@@ -513,7 +539,7 @@ def _check_mx(q: torch.Tensor, scale: torch.Tensor) -> tuple[int, int]:
     if q.dtype != torch.uint8 or scale.dtype != torch.uint8 or q.dim() != 2:
         raise TypeError("an MXFP4 matrix is a uint8 [R, K / 2] tensor of codes and a uint8 tensor of scales")
     R, K = q.shape[0], 2 * q.shape[1]
-    if tuple(scale.shape) != mxfp4_scale_shape(R, K):
+    if scale.shape != mxfp4_scale_shape(R, K):
         raise ValueError(f"scales {tuple(scale.shape)} do not fit a [{R}, {K}] matrix: {mxfp4_scale_shape(R, K)}")
     return R, K
 
@@ -529,8 +555,8 @@ def quantize_mxfp4(t: torch.Tensor):
     if K % 32:
         raise ValueError(f"{K} columns are not a multiple of 32")
     dt = dtype_code(t.dtype)
-    q = torch.empty((R, K // 2), device=dev, dtype=torch.uint8)
-    scale = torch.empty(mxfp4_scale_shape(R, K), device=dev, dtype=torch.uint8)
+    q = t.new_empty((R, K // 2), dtype=torch.uint8)
+    scale = q.new_empty(mxfp4_scale_shape(R, K))
     _launch(dev, "swiglu_b200_quantize_mxfp4", t.data_ptr(), q.data_ptr(), scale.data_ptr(), R, K, dt)
     return q, scale
 
@@ -539,9 +565,9 @@ def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype
     """The [R, K] values of an MXFP4 matrix, in bf16 or f32 (exact)."""
     dev = _check_cuda(q, scale)
     R, K = _check_mx(q, scale)
-    out = torch.empty((R, K), device=dev, dtype=dtype)
-    _launch(dev, "swiglu_b200_dequantize_mxfp4", q.data_ptr(), scale.data_ptr(), out.data_ptr(), R, K,
-            dtype_code(dtype))
+    dt = dtype_code(dtype)
+    out = q.new_empty((R, K), dtype=dtype)
+    _launch(dev, "swiglu_b200_dequantize_mxfp4", q.data_ptr(), scale.data_ptr(), out.data_ptr(), R, K, dt)
     return out
 
 
@@ -554,7 +580,8 @@ def matmul_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_sc
     N, K2 = _check_mx(bq, b_scale)
     if K != K2:
         raise ValueError(f"inner dimensions differ: {K} vs {K2}")
-    out = torch.empty((M, N), device=dev, dtype=out_dtype)
+    dt = dtype_code(out_dtype)
+    out = aq.new_empty((M, N), dtype=out_dtype)
     _launch(dev, "swiglu_b200_matmul_mxfp4", aq.data_ptr(), a_scale.data_ptr(), bq.data_ptr(), b_scale.data_ptr(),
-            out.data_ptr(), M, N, K, dtype_code(out_dtype))
+            out.data_ptr(), M, N, K, dt)
     return out
