@@ -152,6 +152,84 @@ def _(aq, a_scale, bq, b_scale):
     return aq.new_empty((aq.shape[0], bq.shape[0]), dtype=torch.bfloat16)
 
 
+@torch.library.custom_op(f"{_NS}::forward_logic", mutates_args=(), device_types="cuda")
+def forward_logic(preact: torch.Tensor, layout: int) -> torch.Tensor:
+    """h [M, H] = left * silu(gate) of preact [M, 2H]."""
+    return ops.forward_logic(preact, layout=layout)
+
+
+@forward_logic.register_fake
+def _(preact, layout):
+    return preact.new_empty((preact.shape[0], preact.shape[1] // 2))
+
+
+@torch.library.custom_op(f"{_NS}::quantize_mxfp4", mutates_args=(), device_types="cuda")
+def quantize_mxfp4(t: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes [R, K / 2], scale tiles) of a [R, K] matrix."""
+    return ops.quantize_mxfp4(t)
+
+
+@quantize_mxfp4.register_fake
+def _(t):
+    R, K = t.shape
+    return (t.new_empty((R, K // 2), dtype=torch.uint8),
+            t.new_empty(((R + 127) // 128, (K + 127) // 128, 32, 4, 4), dtype=torch.uint8))
+
+
+@torch.library.custom_op(f"{_NS}::matmul_mxfp4", mutates_args=(), device_types="cuda")
+def matmul_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_scale: torch.Tensor) -> torch.Tensor:
+    """A . B^T in bf16 for MXFP4 A [M, K], B [N, K]."""
+    return ops.matmul_mxfp4(aq, a_scale, bq, b_scale)
+
+
+@matmul_mxfp4.register_fake
+def _(aq, a_scale, bq, b_scale):
+    return aq.new_empty((aq.shape[0], bq.shape[0]), dtype=torch.bfloat16)
+
+
+# Without a residual the stream is x itself, which an op may not return: its
+# place holds an empty tensor then.
+@torch.library.custom_op(f"{_NS}::rmsnorm_fwd", mutates_args=(), device_types="cuda")
+def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
+                eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, s, rstd) of the residual RMS norm."""
+    y, s, rstd = ops.rmsnorm_fwd(x, weight, residual, eps=eps)
+    return y, s if residual is not None else x.new_empty(0), rstd
+
+
+@rmsnorm_fwd.register_fake
+def _(x, weight, residual, eps):
+    return (torch.empty_like(x), torch.empty_like(x) if residual is not None else x.new_empty(0),
+            x.new_empty((x.shape[0],), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::rmsnorm_fwd_e4m3", mutates_args=(), device_types="cuda")
+def rmsnorm_fwd_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor],
+                     eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(q e4m3, row scales, s, rstd) of the residual RMS norm."""
+    q, scale, s, rstd = ops.rmsnorm_fwd_e4m3(x, weight, residual, eps=eps)
+    return q, scale, s if residual is not None else x.new_empty(0), rstd
+
+
+@rmsnorm_fwd_e4m3.register_fake
+def _(x, weight, residual, eps):
+    rows = x.new_empty((x.shape[0],), dtype=torch.float32)
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), rows,
+            torch.empty_like(x) if residual is not None else x.new_empty(0), torch.empty_like(rows))
+
+
+@torch.library.custom_op(f"{_NS}::rmsnorm_bwd", mutates_args=(), device_types="cuda")
+def rmsnorm_bwd(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                ds: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight) of the residual RMS norm."""
+    return ops.rmsnorm_bwd(dy, s, weight, rstd, ds)
+
+
+@rmsnorm_bwd.register_fake
+def _(dy, s, weight, rstd, ds):
+    return torch.empty_like(s), torch.empty_like(weight)
+
+
 class _Eager:
     """The calls the Functions make, on the plain ops functions."""
 
@@ -198,6 +276,30 @@ class _Eager:
     def matmul_e4m3(aq, a_scale, bq, b_scale):
         return ops.matmul_e4m3(aq, a_scale, bq, b_scale)
 
+    @staticmethod
+    def forward_logic(preact, layout):
+        return ops.forward_logic(preact, layout=layout)
+
+    @staticmethod
+    def quantize_mxfp4(t):
+        return ops.quantize_mxfp4(t)
+
+    @staticmethod
+    def matmul_mxfp4(aq, a_scale, bq, b_scale):
+        return ops.matmul_mxfp4(aq, a_scale, bq, b_scale)
+
+    @staticmethod
+    def rmsnorm_fwd(x, weight, residual, eps):
+        return ops.rmsnorm_fwd(x, weight, residual, eps=eps)
+
+    @staticmethod
+    def rmsnorm_fwd_e4m3(x, weight, residual, eps):
+        return ops.rmsnorm_fwd_e4m3(x, weight, residual, eps=eps)
+
+    @staticmethod
+    def rmsnorm_bwd(dy, s, weight, rstd, ds):
+        return ops.rmsnorm_bwd(dy, s, weight, rstd, ds)
+
 
 class _Traced:
     """The same calls as registered ops (what Dynamo records)."""
@@ -241,6 +343,32 @@ class _Traced:
     @staticmethod
     def matmul_e4m3(aq, a_scale, bq, b_scale):
         return torch.ops.swiglu_b200.matmul_e4m3(aq, a_scale, bq, b_scale)
+
+    @staticmethod
+    def forward_logic(preact, layout):
+        return torch.ops.swiglu_b200.forward_logic(preact, layout)
+
+    @staticmethod
+    def quantize_mxfp4(t):
+        return torch.ops.swiglu_b200.quantize_mxfp4(t)
+
+    @staticmethod
+    def matmul_mxfp4(aq, a_scale, bq, b_scale):
+        return torch.ops.swiglu_b200.matmul_mxfp4(aq, a_scale, bq, b_scale)
+
+    @staticmethod
+    def rmsnorm_fwd(x, weight, residual, eps):
+        y, s, rstd = torch.ops.swiglu_b200.rmsnorm_fwd(x, weight, residual, eps)
+        return y, x if residual is None else s, rstd
+
+    @staticmethod
+    def rmsnorm_fwd_e4m3(x, weight, residual, eps):
+        q, scale, s, rstd = torch.ops.swiglu_b200.rmsnorm_fwd_e4m3(x, weight, residual, eps)
+        return q, scale, x if residual is None else s, rstd
+
+    @staticmethod
+    def rmsnorm_bwd(dy, s, weight, rstd, ds):
+        return torch.ops.swiglu_b200.rmsnorm_bwd(dy, s, weight, rstd, ds)
 
 
 def kernels():

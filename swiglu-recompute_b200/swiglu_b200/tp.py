@@ -355,6 +355,20 @@ def tp_swiglu(x_local, w1_local, w2_local, group=None, compute=NativeCompute, re
     return _TPSwiGLUFunction.apply(x_local, w1_local, w2_local, group, compute, reduce_f32, fused_rs, chunks)
 
 
+def clip_sharded_grad_norm_(grads, max_norm, device, group=None):
+    """ops.clip_grad_norm_ for gradients that are shards: each rank of `group`
+    passes its own (none, some or all of them), and all are scaled by the norm
+    over all ranks. Returns that norm (f32, on `device`)."""
+    square = torch.zeros((), dtype=torch.float64, device=device)
+    if grads:
+        square = ops.grad_norm(grads).double().square()
+    dist.all_reduce(square, group=group)
+    norm = square.sqrt().float()
+    if grads:
+        ops.clip_grads_by_norm_(grads, norm, max_norm)
+    return norm
+
+
 class SwiGLUMLPTensorParallel(nn.Module):
     """One SwiGLU MLP block split over the ranks of `group` (weights are this
     rank's shards: w1 [2H/t, D], w2 [Dout, H/t])."""
@@ -383,6 +397,15 @@ class SwiGLUMLPTensorParallel(nn.Module):
         self.w1.copy_(shard_w1_rows(w1, self.rank, self.world))
         self.w2.copy_(shard_w2(w2, self.rank, self.world))
         return self
+
+    @torch.no_grad()
+    def clip_grad_norm_(self, max_norm):
+        """Clips this block's gradients by the norm over all ranks' shards: the
+        ranks' squared norms are added in f64 (one all-reduce of one value),
+        then every rank scales its own. Returns that norm. Every rank calls it;
+        one without gradients adds zero."""
+        grads = [p.grad for p in (self.w1, self.w2) if p.grad is not None]
+        return clip_sharded_grad_norm_(grads, max_norm, self.w1.device, self.group)
 
     def forward(self, x_local):
         frs = None

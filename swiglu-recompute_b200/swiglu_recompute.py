@@ -228,6 +228,44 @@ class SwiGLUFP8ForwardFunction(torch.autograd.Function):
         return gx, gw1, gw2
 
 
+class SwiGLUFP4ForwardFunction(torch.autograd.Function):
+    """Forward GEMMs with MXFP4 operands, backward as the recompute Function.
+
+    x, W1, h and W2 are quantised in blocks of 32 along the contraction (e2m1
+    codes, one power-of-two scale a block); preact = x W1^T and y = h W2^T run
+    on the tensor core's block-scaled 4-bit kind with f32 accumulation. preact
+    (bf16) is saved as in SwiGLUMemoryOptimizedFunction, whose bf16 backward
+    follows unchanged. No counterpart in the reference; results differ from the
+    bf16 block by the e2m1 rounding of the four operands (one mantissa bit).
+    """
+
+    @staticmethod
+    def forward(ctx, x, W1, W2):
+        lead = x.shape[:-1]
+        x2 = _flatten_rows(x)
+        W1c, W2c = W1.contiguous(), W2.contiguous()
+        K = kernels()
+        xq, xs = K.quantize_mxfp4(x2)
+        w1q, w1s = K.quantize_mxfp4(W1c)
+        preact = K.matmul_mxfp4(xq, xs, w1q, w1s)
+        del xq, w1q
+        hq, hs = K.quantize_mxfp4(K.forward_logic(preact, LAYOUT_STD))
+        w2q, w2s = K.quantize_mxfp4(W2c)
+        y = K.matmul_mxfp4(hq, hs, w2q, w2s)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(x2, W1c, W2c, preact)
+        ctx.x_shape = x.shape
+        return y.reshape(*lead, W2.shape[0])
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        x, W1, W2, preact = ctx.saved_tensors
+        gx, gw1, gw2 = _recompute_backward(ctx, grad_y, x, W1, W2, preact, w_form=W1_ROWS, layout=LAYOUT_STD)
+        if gx is not None:
+            gx = gx.reshape(ctx.x_shape)
+        return gx, gw1, gw2
+
+
 # -----------------------------------------------------------------------------
 # nn.Module wrapper
 # -----------------------------------------------------------------------------
@@ -263,6 +301,44 @@ class SwiGLUMLPFP8Forward(SwiGLUMLPCustom):
         if x.dtype != torch.bfloat16:
             raise TypeError("the e4m3 forward takes bf16 activations")
         return SwiGLUFP8ForwardFunction.apply(x, self.w1, self.w2)
+
+
+class SwiGLUMLPFP4Forward(SwiGLUMLPCustom):
+    """SwiGLUMLPCustom whose forward GEMMs take MXFP4 operands (bf16 weights and
+    activations quantised on the fly; dim and hidden_dim multiples of 32); bf16
+    recompute backward."""
+
+    def forward(self, x):
+        if x.dtype != torch.bfloat16:
+            raise TypeError("the MXFP4 forward takes bf16 activations")
+        return SwiGLUFP4ForwardFunction.apply(x, self.w1, self.w2)
+
+
+class SwiGLUMLPFP4Inference(nn.Module):
+    """The forward of SwiGLUMLPFP4Forward for serving: only the MXFP4 weights
+    are kept (quantised once, 17/32 of a byte a value), and no gradients. The
+    same results as the training module's forward from the same weights."""
+
+    def __init__(self, w1: torch.Tensor, w2: torch.Tensor):
+        super().__init__()
+        for name, w in (("w1", w1), ("w2", w2)):
+            q, scale = ops.quantize_mxfp4(w.detach().contiguous())
+            self.register_buffer(f"{name}_q", q)
+            self.register_buffer(f"{name}_scale", scale)
+
+    @classmethod
+    def from_mlp(cls, mlp):
+        """From a block with w1 [2H, D] and w2 [Dout, H] on a CUDA device."""
+        return cls(mlp.w1, mlp.w2)
+
+    @torch.no_grad()
+    def forward(self, x):
+        if x.dtype != torch.bfloat16:
+            raise TypeError("the MXFP4 forward takes bf16 activations")
+        K = kernels()
+        preact = K.matmul_mxfp4(*K.quantize_mxfp4(_flatten_rows(x)), self.w1_q, self.w1_scale)
+        y = K.matmul_mxfp4(*K.quantize_mxfp4(K.forward_logic(preact, LAYOUT_STD)), self.w2_q, self.w2_scale)
+        return y.reshape(*x.shape[:-1], y.shape[-1])
 
 
 class SwiGLUMLPGroundTruth(nn.Module):
