@@ -14,8 +14,6 @@ The reference has the MLP alone (swiglu_recompute.py:81-98).
 
 from __future__ import annotations
 
-from types import SimpleNamespace
-
 import torch
 import torch.nn as nn
 
@@ -25,6 +23,15 @@ from swiglu_b200.ops import LAYOUT_STD, W1_ROWS
 from swiglu_recompute import _flatten_rows, _recompute_backward
 
 PRECISIONS = ("bf16", "e4m3", "mxfp4")
+
+
+class _MLPPart:
+    """What _recompute_backward asks of a Function's context, for the MLP inside
+    the block's."""
+
+    def __init__(self, needs_input_grad, consumed):
+        self.needs_input_grad = needs_input_grad
+        self._preact_consumed = consumed
 
 
 def _same_stream(x, residual):
@@ -113,10 +120,11 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
         # The norm's output again: the same kernel on the same rows.
         n = K.rmsnorm_fwd(s, g, None, ctx.eps)[0] if need_w1 else None
         need_n = need_x or need_r or need_g
-        mlp = SimpleNamespace(needs_input_grad=(need_n, need_w1, need_w2),
-                              _preact_consumed=getattr(ctx, "_preact_consumed", False))
+        eager = not torch.compiler.is_compiling()
+        mlp = _MLPPart((need_n, need_w1, need_w2), eager and getattr(ctx, "_preact_consumed", False))
         dn, dw1, dw2 = _recompute_backward(mlp, grad_y, n, W1, W2, preact, w_form=W1_ROWS, layout=LAYOUT_STD)
-        ctx._preact_consumed = mlp._preact_consumed
+        if eager:
+            ctx._preact_consumed = mlp._preact_consumed
         dx = dg = None
         if need_n:
             d2 = None if ds is None else _flatten_rows(ds).to(s.dtype)
