@@ -70,6 +70,17 @@ struct ChunkSlots {
   }
   __device__ __forceinline__ long long at(int i) const { return e0 + i * (kGradThreads * N); }
   __device__ __forceinline__ bool inside(int i) const { return at(i) >= 0 && at(i) + N <= size; }
+  __device__ __forceinline__ uint4 load_one(int i) const {
+    if (inside(i)) return __ldg(reinterpret_cast<const uint4*>(base + at(i)));
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (at(i) + e < 0 || at(i) + e >= size) continue;
+      if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(base[at(i) + e]);
+      else w[e / 2] |= static_cast<uint32_t>(__bfloat16_as_ushort(base[at(i) + e])) << (16 * (e & 1));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
   __device__ __forceinline__ void load(uint4 (&u)[kGradSlots]) const {
     if (whole) {
       const uint4* p = reinterpret_cast<const uint4*>(base + e0);
@@ -77,20 +88,7 @@ struct ChunkSlots {
       for (int i = 0; i < kGradSlots; ++i) u[i] = __ldg(p + i * kGradThreads);
     } else {
 #pragma unroll
-      for (int i = 0; i < kGradSlots; ++i) {
-        if (inside(i)) {
-          u[i] = __ldg(reinterpret_cast<const uint4*>(base + at(i)));
-        } else {
-          uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            if (at(i) + e < 0 || at(i) + e >= size) continue;
-            if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(base[at(i) + e]);
-            else w[e / 2] |= static_cast<uint32_t>(__bfloat16_as_ushort(base[at(i) + e])) << (16 * (e & 1));
-          }
-          u[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+      for (int i = 0; i < kGradSlots; ++i) u[i] = load_one(i);
     }
   }
   __device__ static __forceinline__ void values(const uint4& u, float (&f)[N]) {
@@ -111,23 +109,27 @@ struct ChunkSlots {
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const GradTable& t, int k, int chunk) {
   constexpr int N = ChunkSlots<T>::N;
+  const ChunkSlots<T> slots(t, k, chunk);
   uint4 u[kGradSlots];
-  ChunkSlots<T>(t, k, chunk).load(u);
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  slots.load(u);
+  float2 sum[2] = {};  // packed f32x2 arithmetic
 #pragma unroll
   for (int i = 0; i < kGradSlots; ++i) {
     float f[N];
     ChunkSlots<T>::values(u[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[e & 3] += f[e] * f[e];
+    for (int e = 0; e < N / 2; ++e) {
+      const float2 v = make_float2(f[2 * e], f[2 * e + 1]);
+      sum[e & 1] = __ffma2_rn(v, v, sum[e & 1]);
+    }
   }
-  const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  const float total = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
   if (total >= 1e-30f && total <= 1e37f) return static_cast<double>(total);
   double exact = 0.0;
-#pragma unroll
-  for (int i = 0; i < kGradSlots; ++i) {
+#pragma unroll 1
+  for (int i = 0; i < kGradSlots; ++i) {  // read again, so that the usual path keeps no values
     float f[N];
-    ChunkSlots<T>::values(u[i], f);
+    ChunkSlots<T>::values(slots.load_one(i), f);
 #pragma unroll
     for (int e = 0; e < N; ++e) exact += static_cast<double>(f[e]) * static_cast<double>(f[e]);
   }
@@ -183,7 +185,11 @@ __device__ __forceinline__ void chunk_scale(const GradTable& t, int k, int chunk
     float f[N];
     ChunkSlots<T>::values(u[i], f);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f[e] *= factor;
+    for (int e = 0; e < N / 2; ++e) {
+      const float2 v = __fmul2_rn(make_float2(f[2 * e], f[2 * e + 1]), make_float2(factor, factor));
+      f[2 * e] = v.x;
+      f[2 * e + 1] = v.y;
+    }
     const long long at = slots.at(i);
     if (same && (slots.whole || slots.inside(i))) {
       uint4 r;

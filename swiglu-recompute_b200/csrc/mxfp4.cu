@@ -27,25 +27,45 @@ constexpr int kBlock = 32;          // columns that share a scale
 constexpr int kTileRows = 128;
 constexpr int kTileBytes = kMxTileBytes;
 constexpr int kQuantCols = 256;     // columns of one CTA: a warp covers a row of them, 8 a thread
+constexpr int kQuantRows = 64;      // and its rows
 constexpr int kQuantThreads = 256;
 
 __device__ __forceinline__ float power_of_two(int field) { return __uint_as_float(static_cast<uint32_t>(field) << 23); }
 
-// 2^(byte - 127): byte 0 is the subnormal 2^-127, byte 255 a NaN.
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-  return byte == 0 ? __uint_as_float(0x00400000u) : byte == 255 ? __uint_as_float(0x7fc00000u) : power_of_two(byte);
+// 2^(byte - 127) as two bf16: byte 0 is the subnormal 2^-127, byte 255 a NaN.
+__device__ __forceinline__ uint32_t scale_bf16x2(uint32_t byte) {
+  const uint32_t s = byte == 0 ? 0x0040u : byte == 255 ? 0x7fc0u : byte << 7;
+  return s | (s << 16);
 }
 
-// Two e2m1 codes (low nibble first) as f32.
-__device__ __forceinline__ float2 e2m1x2_value(uint32_t byte) {
-  const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1);
-  return __half22float2(__half2(h));
+// Eight e2m1 codes as bf16 pairs: the seven bits above the sign of a code's value
+// are looked up by byte permutation (two tables of eight bytes), which takes half
+// the instructions of converting through f16 and f32.
+__device__ __forceinline__ void e2m1x8_bf16(uint32_t codes, uint32_t (&out)[4]) {
+  constexpr uint32_t kHigh0 = 0x3f3f3f00u, kHigh1 = 0x40404040u;  // 0 0.5 1 1.5 | 2 3 4 6
+  constexpr uint32_t kLow0 = 0xc0800000u, kLow1 = 0xc0804000u;
+  const uint32_t sel = codes & 0x77777777u;
+  const uint32_t even = (codes << 4) & 0x80808080u, odd = codes & 0x80808080u;  // sign bits of codes 0 2 4 6, 1 3 5 7
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // codes 4h .. 4h + 3
+    const uint32_t pick = h ? sel >> 16 : sel;
+    const uint32_t high = __byte_perm(kHigh0, kHigh1, pick) | __byte_perm(even, odd, h ? 0x7362 : 0x5140);
+    const uint32_t low = __byte_perm(kLow0, kLow1, pick);
+    out[2 * h] = __byte_perm(low, high, 0x5140);
+    out[2 * h + 1] = __byte_perm(low, high, 0x7362);
+  }
 }
 
-// One CTA: 128 rows x 256 columns, two scale tiles. A warp takes a row at a time,
-// 16 bytes a lane (bf16: all 256 columns, four lanes a block; f32: twice 128,
-// eight lanes a block), several rows in flight; the scale bytes are collected in
-// shared memory and leave as whole tiles, none is written alone.
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// One CTA: 64 rows x 256 columns, half of two scale tiles (whole tiles left 13 % of
+// the last round of CTAs idle at 28672 x 3584). A warp takes a row at a time, 16
+// bytes a lane (bf16: all 256 columns, four lanes a block; f32: twice 128, eight
+// lanes a block), several rows in flight; the scale bytes are collected in shared
+// memory and leave eight at a time.
 template <typename T>
 struct MxLanes {
   static constexpr int E = 16 / sizeof(T);             // elements of a lane
@@ -71,41 +91,62 @@ __device__ __forceinline__ uint32_t top_exponent(const uint4& u) {
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kQuantThreads, 4) quantize_mxfp4_kernel(const T* __restrict__ src,
-                                                                          uint8_t* __restrict__ dst,
-                                                                          uint8_t* __restrict__ scale, long long rows,
-                                                                          int cols, int tiles_k) {
+// Where a CTA works, and its scale bytes: [tile of two][row % 32][row / 32 of two][block].
+struct QuantBlock {
+  long long r0;   // first row
+  int c0, warp, lane;
+  long long tile; // first scale tile
+  int half;       // which two of the tile's four groups of 32 rows
+  int tiles;      // scale tiles inside the matrix: 1 or 2
+
+  __device__ __forceinline__ QuantBlock(int cols, int tiles_k) {
+    const int col_blocks = (cols + kQuantCols - 1) / kQuantCols;
+    const long long rb = blockIdx.x / col_blocks;
+    const int cb = static_cast<int>(blockIdx.x % col_blocks);
+    r0 = rb * kQuantRows;
+    c0 = cb * kQuantCols;
+    warp = static_cast<int>(warp_id());
+    lane = static_cast<int>(lane_id());
+    tile = rb / 2 * tiles_k + 2 * cb;
+    half = static_cast<int>(rb % 2);
+    tiles = min(2, tiles_k - 2 * cb);
+  }
+  __device__ __forceinline__ static int byte_of(int row, int block) {
+    return (block >> 2) * 256 + (row & 31) * 8 + (row >> 5) * 4 + (block & 3);
+  }
+  // Thread t < 32 * tiles moves eight bytes of tile t / 32.
+  __device__ __forceinline__ long long at() const {
+    return (tile + (threadIdx.x >> 5)) * kTileBytes + (threadIdx.x & 31) * 16 + half * 8;
+  }
+};
+
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void quantize_rows(const QuantBlock& q, const T* __restrict__ src,
+                                              uint8_t* __restrict__ dst, uint8_t* bytes, long long rows, int cols) {
   using L = MxLanes<T>;
-  __shared__ __align__(16) uint8_t tile[2 * kTileBytes];
-  const int lane = static_cast<int>(lane_id()), warp = static_cast<int>(warp_id());
-  const long long r0 = blockIdx.y * static_cast<long long>(kTileRows) + warp;
-  const int c0 = blockIdx.x * kQuantCols + lane * L::E;
-  reinterpret_cast<uint32_t*>(tile)[threadIdx.x] = 0;
-  __syncthreads();
+  const long long r0 = q.r0 + q.warp, at0 = r0 * cols + q.c0 + q.lane * L::E;
+  const long long step = 8ll * cols;
 #pragma unroll 1
-  for (int i0 = 0; i0 < 16 && r0 + i0 * 8 < rows; i0 += L::BATCH) {
+  for (int i0 = 0; i0 < 8; i0 += L::BATCH) {
     uint4 u[L::BATCH][L::GROUPS];
 #pragma unroll
     for (int i = 0; i < L::BATCH; ++i) {
 #pragma unroll
       for (int g = 0; g < L::GROUPS; ++g) {
-        const long long r = r0 + (i0 + i) * 8;
-        const int c = c0 + g * 32 * L::E;
+        const bool in = WHOLE || (r0 + (i0 + i) * 8 < rows && q.c0 + (g * 32 + q.lane) * L::E < cols);
         u[i][g] = make_uint4(0, 0, 0, 0);
-        if (r < rows && c < cols) u[i][g] = __ldg(reinterpret_cast<const uint4*>(src + r * cols + c));
+        if (in) u[i][g] = __ldg(reinterpret_cast<const uint4*>(src + at0 + (i0 + i) * step + g * 32 * L::E));
       }
     }
 #pragma unroll
     for (int i = 0; i < L::BATCH; ++i) {
 #pragma unroll
       for (int g = 0; g < L::GROUPS; ++g) {
-        const long long r = r0 + (i0 + i) * 8;
-        const int c = c0 + g * 32 * L::E;
         uint32_t field = top_exponent<T>(u[i][g]);  // 127 + floor(log2 max), 0 below the normals
 #pragma unroll
         for (int o = 1; o < L::LANES; o *= 2) field = max(field, __shfl_xor_sync(0xffffffffu, field, o));
-        if (r >= rows || c >= cols) continue;  // cols is a multiple of 32: a block is inside or not
+        // cols is a multiple of 32: a block is inside or not
+        if (!WHOLE && !(r0 + (i0 + i) * 8 < rows && q.c0 + (g * 32 + q.lane) * L::E < cols)) continue;
         const int byte = field == 255 ? 255 : max(static_cast<int>(field) - 2, 0);
         const float inv = power_of_two(254 - min(byte, 253));
         const uint32_t w[4] = {u[i][g].x, u[i][g].y, u[i][g].z, u[i][g].w};
@@ -115,26 +156,75 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_mxfp4_kernel(const 
           float2 v;
           if constexpr (sizeof(T) == 4) v = make_float2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
           else v = unpack_bf16x2(w[e]);
-          const __nv_fp4x2_storage_t q =
-              __nv_cvt_float2_to_fp4x2(make_float2(v.x * inv, v.y * inv), __NV_E2M1, cudaRoundNearest);
-          out |= static_cast<uint32_t>(q) << (8 * e);
+          const __nv_fp4x2_storage_t code =
+              __nv_cvt_float2_to_fp4x2(__fmul2_rn(v, make_float2(inv, inv)), __NV_E2M1, cudaRoundNearest);
+          out |= static_cast<uint32_t>(code) << (8 * e);
         }
-        uint8_t* to = dst + r * (cols / 2) + c / 2;
+        uint8_t* to = dst + (at0 + (i0 + i) * step + g * 32 * L::E) / 2;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(out);
         else *reinterpret_cast<uint32_t*>(to) = out;
-        if (lane % L::LANES == 0) {
-          const int b = (c - static_cast<int>(blockIdx.x) * kQuantCols) / kBlock;  // 0..7 of this CTA's blocks
-          const int rt = (i0 + i) * 8 + warp;
-          tile[(b >> 2) * kTileBytes + (rt & 31) * 16 + (rt >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(byte);
-        }
+        if (q.lane % L::LANES == 0)
+          bytes[QuantBlock::byte_of((i0 + i) * 8 + q.warp, (g * 32 + q.lane) / L::LANES)] = static_cast<uint8_t>(byte);
       }
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads, 4) quantize_mxfp4_kernel(const T* __restrict__ src,
+                                                                          uint8_t* __restrict__ dst,
+                                                                          uint8_t* __restrict__ scale, long long rows,
+                                                                          int cols, int tiles_k) {
+  __shared__ __align__(16) uint8_t bytes[512];
+  const QuantBlock q(cols, tiles_k);
+  if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(bytes)[threadIdx.x] = 0;
   __syncthreads();
-  const int t = 2 * blockIdx.x + (threadIdx.x >> 5);
-  if (threadIdx.x < 64 && t < tiles_k) {
-    uint8_t* to = scale + (blockIdx.y * static_cast<long long>(tiles_k) + t) * kTileBytes;
-    reinterpret_cast<uint4*>(to)[threadIdx.x & 31] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
+  // Blocks wholly inside the matrix skip the checks.
+  if (q.r0 + kQuantRows <= rows && q.c0 + kQuantCols <= cols)
+    quantize_rows<T, true>(q, src, dst, bytes, rows, cols);
+  else
+    quantize_rows<T, false>(q, src, dst, bytes, rows, cols);
+  __syncthreads();
+  if (threadIdx.x < 32 * q.tiles)
+    *reinterpret_cast<uint2*>(scale + q.at()) = reinterpret_cast<const uint2*>(bytes)[threadIdx.x];
+}
+
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void dequantize_rows(const QuantBlock& q, const uint8_t* __restrict__ src, uint2 tile,
+                                                uint8_t* bytes, T* __restrict__ dst, long long rows, int cols) {
+  using L = MxLanes<T>;
+  const long long r0 = q.r0 + q.warp, at0 = r0 * cols + q.c0 + q.lane * L::E;
+  const long long step = 8ll * cols;
+  uint32_t codes[8][L::GROUPS];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int g = 0; g < L::GROUPS; ++g) {
+      if (!WHOLE && !(r0 + i * 8 < rows && q.c0 + (g * 32 + q.lane) * L::E < cols)) continue;
+      const uint8_t* from = src + (at0 + i * step + g * 32 * L::E) / 2;
+      if constexpr (sizeof(T) == 4) codes[i][g] = __ldg(reinterpret_cast<const uint16_t*>(from));
+      else codes[i][g] = __ldg(reinterpret_cast<const uint32_t*>(from));
+    }
+  }
+  if (threadIdx.x < 64) reinterpret_cast<uint2*>(bytes)[threadIdx.x] = tile;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int g = 0; g < L::GROUPS; ++g) {
+      if (!WHOLE && !(r0 + i * 8 < rows && q.c0 + (g * 32 + q.lane) * L::E < cols)) continue;
+      const uint32_t s = scale_bf16x2(bytes[QuantBlock::byte_of(i * 8 + q.warp, (g * 32 + q.lane) / L::LANES)]);
+      uint32_t w[4];
+      e2m1x8_bf16(codes[i][g], w);
+      if constexpr (sizeof(T) == 4) {  // four codes
+        const uint32_t a = mul_bf16x2(w[0], s), b = mul_bf16x2(w[1], s);
+        w[0] = a << 16, w[1] = a & 0xffff0000u, w[2] = b << 16, w[3] = b & 0xffff0000u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = mul_bf16x2(w[e], s);
+      }
+      *reinterpret_cast<uint4*>(dst + at0 + i * step + g * 32 * L::E) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
@@ -143,54 +233,14 @@ __global__ void __launch_bounds__(kQuantThreads, 4) dequantize_mxfp4_kernel(cons
                                                                             const uint8_t* __restrict__ scale,
                                                                             T* __restrict__ dst, long long rows,
                                                                             int cols, int tiles_k) {
-  using L = MxLanes<T>;
-  __shared__ __align__(16) uint8_t tile[2 * kTileBytes];
-  const int lane = static_cast<int>(lane_id()), warp = static_cast<int>(warp_id());
-  const long long r0 = blockIdx.y * static_cast<long long>(kTileRows) + warp;
-  const int c0 = blockIdx.x * kQuantCols + lane * L::E;
-  const int t = 2 * blockIdx.x + (threadIdx.x >> 5);
-  if (threadIdx.x < 64 && t < tiles_k) {
-    const uint8_t* from = scale + (blockIdx.y * static_cast<long long>(tiles_k) + t) * kTileBytes;
-    reinterpret_cast<uint4*>(tile)[threadIdx.x] = __ldg(reinterpret_cast<const uint4*>(from) + (threadIdx.x & 31));
-  }
-  uint32_t q[16][L::GROUPS];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-#pragma unroll
-    for (int g = 0; g < L::GROUPS; ++g) {
-      const long long r = r0 + i * 8;
-      const int c = c0 + g * 32 * L::E;
-      if (r < rows && c < cols) {
-        const uint8_t* from = src + r * (cols / 2) + c / 2;
-        if constexpr (sizeof(T) == 4) q[i][g] = __ldg(reinterpret_cast<const uint16_t*>(from));
-        else q[i][g] = __ldg(reinterpret_cast<const uint32_t*>(from));
-      }
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-#pragma unroll
-    for (int g = 0; g < L::GROUPS; ++g) {
-      const long long r = r0 + i * 8;
-      const int c = c0 + g * 32 * L::E;
-      if (r >= rows || c >= cols) continue;
-      const int b = (c - static_cast<int>(blockIdx.x) * kQuantCols) / kBlock, rt = i * 8 + warp;
-      const float s = scale_value(tile[(b >> 2) * kTileBytes + (rt & 31) * 16 + (rt >> 5) * 4 + (b & 3)]);
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < L::E / 2; ++e) {
-        const float2 v = e2m1x2_value((q[i][g] >> (8 * e)) & 0xffu);
-        if constexpr (sizeof(T) == 4) {
-          w[2 * e] = __float_as_uint(v.x * s);
-          w[2 * e + 1] = __float_as_uint(v.y * s);
-        } else {
-          w[e] = pack_bf16x2(v.x * s, v.y * s);
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + r * cols + c) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
+  __shared__ __align__(16) uint8_t bytes[512];
+  const QuantBlock q(cols, tiles_k);
+  uint2 tile = make_uint2(0, 0);
+  if (threadIdx.x < 32 * q.tiles) tile = __ldg(reinterpret_cast<const uint2*>(scale + q.at()));
+  if (q.r0 + kQuantRows <= rows && q.c0 + kQuantCols <= cols)
+    dequantize_rows<T, true>(q, src, tile, bytes, dst, rows, cols);
+  else
+    dequantize_rows<T, false>(q, src, tile, bytes, dst, rows, cols);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -199,14 +249,15 @@ int check_mx(const char* what, int64_t rows, int64_t cols) {
   if (int rc = check_dims(what, rows, cols, 0)) return rc;
   if (cols % kBlock)
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: %lld columns are not a multiple of 32", what, (long long)cols);
-  if ((rows + kTileRows - 1) / kTileRows > 65535)
-    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: more than 8,388,480 rows", what);
+  const int64_t blocks = (rows + kQuantRows - 1) / kQuantRows * ((cols + kQuantCols - 1) / kQuantCols);
+  if (blocks > 0x7ffffffe) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: the matrix is too large", what);
   return SWIGLU_OK;
 }
 
-dim3 quant_grid(int64_t rows, int64_t cols) {
-  return dim3(static_cast<unsigned>((cols + kQuantCols - 1) / kQuantCols),
-              static_cast<unsigned>((rows + kTileRows - 1) / kTileRows));
+// Whole scale tiles: an even number of row blocks, so that the bytes of rows
+// beyond the matrix are written too.
+unsigned quant_grid(int64_t rows, int64_t cols) {
+  return static_cast<unsigned>((rows + kTileRows - 1) / kTileRows * 2 * ((cols + kQuantCols - 1) / kQuantCols));
 }
 
 int op_quantize(const void* src, void* dst, void* scale, int64_t rows, int64_t cols, int dtype, cudaStream_t st) {

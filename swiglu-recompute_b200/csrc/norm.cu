@@ -52,6 +52,14 @@ __device__ __forceinline__ void get16(const uint4& u, float (&f)[kV<T>]) {
     }
   }
 }
+// The same as pairs.
+template <typename T>
+__device__ __forceinline__ void pairs16(const uint4& u, float2 (&f)[kV<T> / 2]) {
+  float v[kV<T>];
+  get16<T>(u, v);
+#pragma unroll
+  for (int i = 0; i < kV<T> / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
 template <typename T>
 __device__ __forceinline__ uint4 set16(const float (&f)[kV<T>]) {
   if constexpr (sizeof(T) == 2)
@@ -316,6 +324,8 @@ struct BwdParams {
   int chunks;         // row chunks of the column pass
   int rows_per_chunk;
   int period;         // rows after which a row's 16-byte offset repeats
+  int stages;         // rows in the shared-memory ring
+  uint32_t* status;   // device error word
 };
 
 // Threads of a backward row, and the registers its three loads take: up to 12,
@@ -444,6 +454,154 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdLoadRegs<VPT> <= 12 ? 2 : 1)
   }
 }
 
+// The same for rows of whole packs that a block shares (more than a warp): rows
+// arrive through a ring of `stages` rows in shared memory, filled by bulk copies,
+// so that what is in flight does not depend on the registers left (11136 x 3584
+// bf16: registers 60.5 us, ring 56.1; 16384 x 8192: 192, 162; 5000 x 16384: 208,
+// 120; 11136 x 3584 f32: 136, 96).
+constexpr int kMaxStages = 8;
+
+template <typename T, typename W, int VPT>
+__global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_ring_kernel(const BwdParams p) {
+  constexpr int V = kV<T>;
+  extern __shared__ __align__(128) uint8_t ring[];  // [stage][dy, s, ds][cols]
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ float sums[2][32];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.cols) * sizeof(T);
+  const uint32_t stage_bytes = row_bytes * (p.ds ? 3 : 2);
+  const int packs = p.cols / V, warps = static_cast<int>(blockDim.x >> 5);
+  const long long step = gridDim.x;
+  auto fill = [&](int stage, long long row) {  // one thread
+    if (row >= p.rows) return;
+    const long long at = row * row_bytes;
+    uint8_t* to = ring + stage * stage_bytes;
+    mbar_arrive_expect_tx(&full[stage], stage_bytes);
+    bulk_load(to, static_cast<const uint8_t*>(p.dy) + at, row_bytes, &full[stage]);
+    bulk_load(to + row_bytes, static_cast<const uint8_t*>(p.s) + at, row_bytes, &full[stage]);
+    if (p.ds) bulk_load(to + 2 * row_bytes, static_cast<const uint8_t*>(p.ds) + at, row_bytes, &full[stage]);
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    for (int i = 0; i < p.stages; ++i) fill(i, blockIdx.x + i * step);
+  }
+  // Pairs of columns: the arithmetic is on packed f32x2 instructions (the kernel
+  // is bound by the instructions it issues, 67 % of the slots without them).
+  constexpr int P = V / 2;
+  const RowPacks<T, false> first(0, p.cols);
+  float2 w[VPT][P], acc[VPT][P];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
+    float f[V] = {};
+    if (k < packs) first.weight(static_cast<const W*>(p.weight), k, f);
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      w[i][e] = make_float2(f[2 * e], f[2 * e + 1]);
+      acc[i][e] = make_float2(0.0f, 0.0f);
+    }
+  }
+  __syncthreads();
+  const float inv = 1.0f / static_cast<float>(p.cols);
+  int stage = 0, buf = 0;
+  uint32_t parity = 0;
+  float next_rstd = blockIdx.x < p.rows ? p.rstd[blockIdx.x] : 0.0f;
+  for (long long row = blockIdx.x; row < p.rows; row += step) {
+    const float rstd = next_rstd;
+    const float2 rstd2 = make_float2(rstd, rstd);
+    if (row + step < p.rows) next_rstd = p.rstd[row + step];
+    const bool ok = mbar_wait(&full[stage], parity, abort_flag, p.status, kErrTimeoutProducer);
+    const uint4* at = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
+    // Four packs stay as loaded and are taken apart twice: as f32 they would spill.
+    constexpr bool kKeep = VPT <= 2;
+    float2 g[kKeep ? VPT : 1][P], v[kKeep ? VPT : 1][P];
+    uint4 dys[kKeep ? 1 : VPT], ss[kKeep ? 1 : VPT], ds[VPT];
+    float2 dot2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
+      if (k >= packs) continue;
+      const int m = kKeep ? i : 0;
+      const uint4 a = at[k], b = at[packs + k];
+      if constexpr (!kKeep) dys[i] = a, ss[i] = b;
+      pairs16<T>(a, g[m]);
+      pairs16<T>(b, v[m]);
+      if (p.ds) ds[i] = at[2 * packs + k];
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const float2 gv = __fmul2_rn(g[m][e], v[m][e]);
+        dot2 = __ffma2_rn(gv, w[i][e], dot2);
+        acc[i][e] = __ffma2_rn(gv, rstd2, acc[i][e]);
+      }
+    }
+    float dot = dot2.x + dot2.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (lane_id() == 0) sums[buf][warp_id()] = dot;
+    // Everybody has read the stage after this barrier, and knows whether it came.
+    if (__syncthreads_or(!ok)) break;
+    if (threadIdx.x == 0) fill(stage, row + p.stages * step);
+    dot = static_cast<int>(lane_id()) < warps ? sums[buf][lane_id()] : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    buf ^= 1;  // a warp may still be reading the other half
+    const float c = -(dot * inv * rstd * rstd) * rstd;
+    const float2 c2 = make_float2(c, c);
+    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + row * p.cols);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
+      if (k >= packs) continue;
+      const int m = kKeep ? i : 0;
+      if constexpr (!kKeep) {
+        pairs16<T>(dys[i], g[m]);
+        pairs16<T>(ss[i], v[m]);
+      }
+      float2 d[P] = {};
+      if (p.ds) pairs16<T>(ds[i], d);
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        d[e] = __ffma2_rn(v[m][e], c2, d[e]);
+        d[e] = __ffma2_rn(__fmul2_rn(g[m][e], rstd2), w[i][e], d[e]);
+      }
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        f[2 * e] = d[e].x;
+        f[2 * e + 1] = d[e].y;
+      }
+      out[k] = set16<T>(f);
+    }
+    if (++stage == p.stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+  if (*abort_flag) {
+    // A copy never came: let the others land before the shared memory goes.
+    if (threadIdx.x == 0) {
+      volatile int never = 0;
+      for (int i = 0; i < p.stages; ++i)
+        if (i != stage) mbar_wait(&full[i], i < stage ? parity ^ 1 : parity, &never, p.status, kErrTimeoutTeardown);
+    }
+    __syncthreads();
+  }
+  float* part = p.partial + blockIdx.x * static_cast<long long>(p.cols);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
+    if (k >= packs) continue;
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      part[k * V + 2 * e] = acc[i][e].x;
+      part[k * V + 2 * e + 1] = acc[i][e].y;
+    }
+  }
+}
+
 // The pair of kernels for any width and alignment. dot_r = sum_j dy_j w_j s_j, a
 // block per row.
 template <typename T, typename W>
@@ -490,6 +648,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_dweight_kernel(const float* part
   const int j = blockIdx.x * 32 + threadIdx.x;
   float acc = 0.0f;
   if (j < cols) {
+#pragma unroll 4
     for (int c = threadIdx.y; c < chunks; c += 32) acc += partial[c * static_cast<long long>(cols) + j];
   }
   part[threadIdx.y][threadIdx.x] = acc;
@@ -618,8 +777,42 @@ bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   return true;
 }
 
+// Rows of 128 packs or more, at least two of them in the ring: 210 KB of shared memory an SM over the blocks its registers hold.
+template <typename T, typename W, int VPT>
+bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
+  const int64_t threads = (p.cols / kV<T> + VPT - 1) / VPT;
+  // (60000 x 512 bf16, 64 packs: registers 55.8 us, ring 67.2.)
+  if (p.cols / kV<T> < 128 || threads > kBwdThreads) return false;
+  const int x = threads_for(threads, kBwdThreads);
+  int64_t per_sm = (VPT == 1 ? 1024 : 512) / x;
+  const int64_t most = most_bwd_blocks(p.rows, p.cols, d.sms);
+  if (per_sm * d.sms > most) per_sm = (most + d.sms - 1) / d.sms;
+  const int64_t stage_bytes = p.cols * sizeof(T) * (p.ds ? 3 : 2);
+  int64_t stages = 210 * 1024 / per_sm / stage_bytes;
+  if (stages < 2) return false;
+  p.stages = static_cast<int>(stages > kMaxStages ? kMaxStages : stages);
+  const int64_t grid = per_sm * d.sms < most ? per_sm * d.sms : most;
+  if (p.rows < 3 * grid) return false;  // a ring pays once a block has several rows to go through
+  p.chunks = static_cast<int>(grid);
+  constexpr auto kern = rmsnorm_bwd_ring_kernel<T, W, VPT>;
+  KernelState& ks = kernel_state<kern>();
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ks.ready.load() & (1ull << dev))) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 212 * 1024) != cudaSuccess) return false;
+    ks.ready.fetch_or(1ull << dev);
+  }
+  kern<<<p.chunks, x, p.stages * stage_bytes, st>>>(p);
+  return true;
+}
+
 template <typename T, typename W, bool SHIFT>
 bool launch_bwd_rows(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
+  if constexpr (!SHIFT) {
+    // Two packs a thread first: 11136 x 3584 bf16 56.5 us (one 59.5, four 60.9).
+    if (launch_bwd_ring<T, W, 2>(p, d, st) || launch_bwd_ring<T, W, 1>(p, d, st) || launch_bwd_ring<T, W, 4>(p, d, st))
+      return true;
+  }
   return launch_bwd_row<T, W, 1, SHIFT>(p, d, st) || launch_bwd_row<T, W, 2, SHIFT>(p, d, st) ||
          launch_bwd_row<T, W, 4, SHIFT>(p, d, st);
 }
@@ -676,6 +869,7 @@ int op_rmsnorm_bwd(BwdParams p, int64_t rows, int64_t cols, int dtype, int weigh
   if (workspace_floats < bwd_floats(rows, cols, d->sms))
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "rmsnorm_bwd: workspace of %lld floats, %lld needed",
                 (long long)workspace_floats, (long long)bwd_floats(rows, cols, d->sms));
+  p.status = d->status;
   p.dot = workspace;
   p.partial = workspace + rows;
   if (dtype == SWIGLU_F32)
@@ -717,7 +911,7 @@ int swiglu_b200_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int num_sms, i
 int swiglu_b200_rmsnorm_bwd(const void* dy, const void* s, const void* weight, const float* rstd, const void* ds,
                             void* dx, void* dweight, float* workspace, int64_t workspace_floats, int64_t rows,
                             int64_t cols, int dtype, int weight_dtype, void* stream) {
-  BwdParams p{dy, s, weight, rstd, ds, dx, nullptr, nullptr, dweight, 0, 0, 0, 0, 1};
+  BwdParams p{dy, s, weight, rstd, ds, dx, nullptr, nullptr, dweight, 0, 0, 0, 0, 1, 0, nullptr};
   return op_rmsnorm_bwd(p, rows, cols, dtype, weight_dtype, workspace, workspace_floats,
                         static_cast<cudaStream_t>(stream));
 }

@@ -345,11 +345,15 @@ def _launch(dev: torch.device, name: str, *args) -> None:
     """`name(*args, stream)` with `dev` current, on its current torch stream."""
     index = dev.index
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
-        _call(dev, name, *args, stream)
-    else:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(dev):
             _call(dev, name, *args, stream)
+    elif _trace is not None:
+        _call(dev, name, *args, stream)
+    else:
+        status = getattr(_lib.load(), name)(*args, stream)
+        if status:
+            _lib.check(status)
 
 
 @lru_cache(maxsize=None)
@@ -410,7 +414,7 @@ def rmsnorm_fwd(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     s = x if residual is None else torch.empty_like(x)
     rstd = x.new_empty(M, dtype=torch.float32)
     _launch(dev, "swiglu_b200_rmsnorm_fwd", x.data_ptr(), _ptr(residual), weight.data_ptr(), y.data_ptr(),
-            s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(eps)), dt, wdt)
+            s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(float(eps))), dt, wdt)
     return y, s, rstd
 
 
@@ -424,7 +428,7 @@ def rmsnorm_fwd_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     s = x if residual is None else torch.empty_like(x)
     rstd = torch.empty_like(scale)
     _launch(dev, "swiglu_b200_rmsnorm_fwd_e4m3", x.data_ptr(), _ptr(residual), weight.data_ptr(), q.data_ptr(),
-            scale.data_ptr(), s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(eps)), dt, wdt)
+            scale.data_ptr(), s.data_ptr(), rstd.data_ptr(), M, D, ctypes.byref(ctypes.c_float(float(eps))), dt, wdt)
     return q, scale, s, rstd
 
 
@@ -510,7 +514,7 @@ def clip_grad_norm_(tensors, max_norm: float, *, out=None) -> torch.Tensor:
     g = _GradList(tensors, out)
     norm = g.norm()
     ws = g.workspace()
-    _launch(g.dev, "swiglu_b200_clip_grad_norm", *g.args(True), ctypes.byref(ctypes.c_double(max_norm)),
+    _launch(g.dev, "swiglu_b200_clip_grad_norm", *g.args(True), ctypes.byref(ctypes.c_double(float(max_norm))),
             ws.data_ptr(), ws.numel(), norm.data_ptr())
     g.written()
     return norm
@@ -523,7 +527,7 @@ def clip_grads_by_norm_(tensors, norm: torch.Tensor, max_norm: float, *, out=Non
     if norm.device != g.dev or norm.dtype != torch.float32 or norm.numel() != 1:
         raise ValueError("norm must be one f32 value on the gradients' device")
     _launch(g.dev, "swiglu_b200_clip_grads_by_norm", *g.args(True), norm.data_ptr(),
-            ctypes.byref(ctypes.c_double(max_norm)))
+            ctypes.byref(ctypes.c_double(float(max_norm))))
     g.written()
 
 

@@ -90,7 +90,7 @@ def test_mxfp4_refusals(lib):
         _said(lib, f(P, P, P, 4, 64, 3, None), 1, b"dtype")
         _said(lib, f(P, None, P, 4, 64, 1, None), 1, b"null")
         _said(lib, f(P + 8, P, P, 4, 64, 1, None), 2, b"16-byte")
-        _said(lib, f(P, P, P, 1 << 30, 64, 1, None), 1, b"rows")
+        _said(lib, f(P, P, P, 1 << 30, 1 << 20, 1, None), 1, b"too large")
         assert f(None, None, None, 0, 64, 1, None) == 0
     _said(lib, m(P, P, P, P, P, 4, 8, 48, 1, None), 1, b"multiple of 32")
     _said(lib, m(P, P, P, P, P, 4, 12, 64, 1, None), 1, b"multiple of 8")
