@@ -450,6 +450,17 @@ def rmsnorm_bwd(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd: t
 
 
 # --------------------------------------------------- gradient norm and clipping
+def _check_dense(t: torch.Tensor, dev: torch.device) -> None:
+    """Raises unless t's values fill one stretch of memory of `dev`, in whatever
+    order of dimensions."""
+    if not t.is_cuda:
+        raise ValueError("swiglu_b200 kernels take CUDA tensors (there is no CPU path)")
+    if t.device != dev:
+        raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
+    if not t.permute(sorted(range(t.dim()), key=t.stride, reverse=True)).is_contiguous():
+        raise ValueError("a gradient's values must fill one stretch of memory")
+
+
 class _GradList:
     """Host arrays of a list of gradients, checked."""
 
@@ -460,7 +471,7 @@ class _GradList:
         dev = self.dev = tensors[0].device
         for t in tensors:
             if t.device != dev or not t.is_cuda or not t.is_contiguous():
-                _check_cuda(tensors[0], t)  # raises with what is wrong
+                _check_dense(t, dev)
         try:
             self.dtypes = array("i", [_CODES[t.dtype] for t in tensors])
         except KeyError as e:
@@ -475,8 +486,10 @@ class _GradList:
             for t, o in zip(tensors, out):
                 if o.shape != t.shape or o.dtype != t.dtype:
                     raise ValueError("an output differs from its gradient in shape or dtype")
-                if o.device != dev or not o.is_contiguous():
-                    _check_cuda(t, o)
+                if o.device != dev or not o.is_contiguous() or not t.is_contiguous():
+                    _check_dense(o, dev)
+                    if o.stride() != t.stride():
+                        raise ValueError("an output's strides differ from its gradient's")
             self.outs = array("Q", [o.data_ptr() for o in out])
 
     def args(self, with_outs: bool):
@@ -498,7 +511,8 @@ class _GradList:
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm (f32, a 0-dim tensor on their device) of all the values of a
-    list of contiguous bf16 / f32 tensors on one device."""
+    list of bf16 / f32 tensors on one device (contiguous in some order of their
+    dimensions)."""
     g = _GradList(tensors)
     norm = g.norm()
     ws = g.workspace()

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from swiglu_b200 import ops
 from swiglu_b200.library import kernels
@@ -57,6 +58,7 @@ class RMSNormResidualFunction(torch.autograd.Function):
         return y if residual is None else (y, s.reshape(x.shape))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, ds=None):
         s, w, rstd = ctx.saved_tensors
         if dy is None:
@@ -111,6 +113,7 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
         return y if residual is None else (y, s.reshape(x.shape))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_y, ds=None):
         s, g, rstd, W1, W2, preact = ctx.saved_tensors
         need_x, need_r, need_g, need_w1, need_w2 = ctx.needs_input_grad[:5]

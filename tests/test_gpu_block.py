@@ -132,12 +132,25 @@ def test_leading_dimensions_partial_gradients_and_second_backward():
     y, s = m(xd, r3)
     (ds,) = torch.autograd.grad(s, [xd], gs.view(3, 4, 5, 64).to(DEV))
     assert torch.equal(ds.view(60, 64).cpu(), gs)
+    # no second derivative, and it says so
+    y, s = m(xd, r3)
+    (dx,) = torch.autograd.grad(y, [xd], gy.view(3, 4, 5, 64).to(DEV), create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
     # weights alone
     y, s = m(x3, r3)
     dg, dw1 = torch.autograd.grad(y, [m.norm_weight, m.w1], gy.view(3, 4, 5, 64).to(DEV))
     assert dg.shape == (64,) and torch.isfinite(dw1).all()
     with torch.no_grad():
         assert torch.equal(m(x3, r3)[0], y.detach())
+
+
+@pytest.mark.parametrize("precision", SB.PRECISIONS)
+def test_no_rows(precision):
+    m, x, r, gy, gs = _make(4, 64, 128, 64, precision=precision)
+    with torch.no_grad():
+        y, s = m(x[:0].to(DEV), r[:0].to(DEV))
+    assert y.shape == (0, 64) and s.shape == (0, 64)
 
 
 def test_norm_module():
@@ -232,6 +245,41 @@ def test_a_training_step_of_two_blocks(precision):
         assert torch.all((got.cpu().double() - want).abs() <= (2 ** -8 + 2.0 ** -18) * want.abs())
     again = step()
     assert torch.equal(again[1], norm) and all(torch.equal(a, b) for a, b in zip(again[0], before))
+    assert ops.device_status(0) == 0
+
+
+@pytest.mark.parametrize("precision", SB.PRECISIONS)
+def test_a_step_captured_in_a_graph(precision):
+    """Forward, gradients and clipping of a block in one CUDA graph, replayed on
+    other inputs: the eager call's bits (at this size no GEMM splits its tail)."""
+    m, x, r, gy, gs = _make(160, 128, 256, 128, precision=precision)
+    params = list(m.parameters())
+    xs, rs, gys = x.to(DEV), r.to(DEV), gy.to(DEV)
+
+    def step(a, b, g):
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        y, s = m(a, b)
+        grads = torch.autograd.grad([y, s], [a, b] + params, [g, g])
+        return (y, s, ops.clip_grad_norm_(grads[2:], 0.1), *grads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(xs, rs, gys)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(xs, rs, gys)
+    for seed in (1, 2):
+        g = torch.Generator().manual_seed(seed)
+        new = [torch.randn(t.shape, generator=g).to(BF).to(DEV) for t in (xs, rs, gys)]
+        want = [t.detach().clone() for t in step(*new)]
+        for a, b in zip((xs, rs, gys), new):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
     assert ops.device_status(0) == 0
 
 

@@ -121,6 +121,41 @@ def test_in_place_bumps_the_version_and_runs_in_a_graph():
     assert n == first and all(torch.equal(a, b) for a, b in zip(ts, clipped))
 
 
+def test_dense_tensors_of_any_dimension_order():
+    src = torch.randn(40, 30, 7)
+    t = src.to(DEV).permute(2, 0, 1)
+    u = src.to(BF).to(DEV).transpose(0, 1)
+    rn, (r, ru) = O.clip([src, src.to(BF)], 2.0)
+    n = ops.clip_grad_norm_([t, u], 2.0)
+    assert abs(n.cpu().double() - rn) <= NORM_TOL * rn
+    assert torch.all((t.permute(1, 2, 0).cpu().double() - r).abs() <= (NORM_TOL + 4 * U) * r.abs())
+    assert torch.all((u.transpose(0, 1).cpu().double() - ru).abs() <= (2 ** -8 + NORM_TOL + 2 * U) * ru.abs())
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm_([t], 1.0, out=[torch.empty(7, 40, 30, device=DEV)])     # other strides
+    for bad in (t[:, ::2], torch.ones(1, device=DEV).expand(5)):
+        with pytest.raises(ValueError):
+            ops.grad_norm([bad])
+
+
+def test_two_streams_at_once():
+    lists = [[torch.randn(300000, device=DEV), torch.randn(1000, 77, device=DEV).to(BF)] for _ in range(2)]
+    want = [ops.grad_norm(ts) for ts in lists]
+    outs = [[torch.empty_like(t) for t in ts] for ts in lists]
+    ref = [[torch.empty_like(t) for t in ts] for ts in lists]
+    for ts, o in zip(lists, ref):
+        ops.clip_grad_norm_(ts, 1.0, out=o)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, ts, o in zip(streams, lists, outs):
+            with torch.cuda.stream(st):
+                got.append(ops.clip_grad_norm_(ts, 1.0, out=o))
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert got[k] == want[k] and all(torch.equal(a, b) for a, b in zip(outs[k], ref[k]))
+
+
 def test_refusals():
     t = torch.ones(64, device=DEV)
     with pytest.raises(ValueError):

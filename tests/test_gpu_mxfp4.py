@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from oracle import operators as O
-from swiglu_b200 import ops
+from swiglu_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -88,7 +88,8 @@ def _check(c, av, bv, out):
 @pytest.mark.parametrize("M,N,K", [(1, 8, 32), (1, 3584, 3584), (2, 128, 64), (3, 136, 96), (7, 256, 14336), (16, 1000, 1056),
                                    (17, 520, 2048), (33, 3584, 544), (64, 264, 3616), (65, 128, 256), (100, 2816, 1024),
                                    (128, 512, 512), (129, 776, 288), (256, 256, 256), (333, 1000, 1440), (512, 3584, 1024),
-                                   (700, 1032, 736), (1025, 520, 320), (2048, 2816, 1024), (4096, 1024, 2816)])
+                                   (700, 1032, 736), (1025, 520, 320), (2048, 2816, 1024), (4096, 1024, 2816), (3000, 8, 64),
+                                   (300, 16, 32), (9, 16392, 96), (130, 40, 8192), (20000, 72, 32)])
 @pytest.mark.parametrize("out", [BF, F32])
 def test_product(M, N, K, out):
     _check(*_product(M, N, K, out), out)
@@ -126,6 +127,44 @@ def test_product_is_run_to_run_identical_and_runs_elsewhere():
         torch.cuda.synchronize()
         assert torch.equal(first, second) and torch.equal(first, third)
     assert ops.device_status(0) == 0
+
+
+def test_two_streams_at_once_and_a_reserve():
+    mats = []
+    for k, (M, N, K) in enumerate([(40, 1024, 4096), (700, 1032, 1056)]):
+        a, b = _matrix(M, K, BF, k).to(DEV), _matrix(N, K, BF, 9 + k).to(DEV)
+        mats.append((*ops.quantize_mxfp4(a), *ops.quantize_mxfp4(b)))
+    want = [ops.matmul_mxfp4(*m) for m in mats]
+    streams = [torch.cuda.Stream() for _ in mats]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for st, m in zip(streams, mats):
+            with torch.cuda.stream(st):
+                got.append(ops.matmul_mxfp4(*m))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _lib.set_sm_reserve(40)
+    try:
+        for m, w in zip(mats, want):
+            assert torch.allclose(ops.matmul_mxfp4(*m).float(), w.float(), rtol=2 ** -6,
+                                  atol=2 ** -6 * w.float().abs().max().item())
+    finally:
+        _lib.set_sm_reserve(0)
+    assert ops.device_status(0) == 0
+
+
+def test_scale_bytes_of_rows_beyond_the_matrix_do_not_matter():
+    for M, N, K in [(5, 24, 128), (300, 520, 256)]:
+        a, b = _matrix(M, K, BF).to(DEV), _matrix(N, K, BF, 1).to(DEV)
+        aq, asc = ops.quantize_mxfp4(a)
+        bq, bsc = ops.quantize_mxfp4(b)
+        want = ops.matmul_mxfp4(aq, asc, bq, bsc)
+        for sc, rows in ((asc, M), (bsc, N)):
+            r = torch.arange(sc.shape[0] * 128, device=DEV)
+            r = r[r >= rows]
+            sc[r // 128, :, r % 32, (r % 128) // 32, :] = 255
+        assert torch.equal(ops.matmul_mxfp4(aq, asc, bq, bsc), want)
 
 
 def test_empty_and_refusals():
