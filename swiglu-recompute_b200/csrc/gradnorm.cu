@@ -150,6 +150,7 @@ __device__ __forceinline__ double block_sum(double v) {
 
 __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
     grad_squares_kernel(const __grid_constant__ GradTable t, double* partial) {
+  wait_for_previous();
   double sum = 0.0;
   const int chunks = t.first_chunk[t.count];
   int k = blockIdx.x < chunks ? tensor_of(t, blockIdx.x) : 0;
@@ -168,6 +169,7 @@ __device__ __forceinline__ double total_norm(const double* partial, int count) {
 }
 
 __global__ void __launch_bounds__(kGradThreads) grad_norm_kernel(const double* partial, int count, float* norm) {
+  wait_for_previous();
   const double n = total_norm(partial, count);
   if (threadIdx.x == 0) *norm = static_cast<float>(n);
 }
@@ -219,6 +221,7 @@ __device__ __forceinline__ void chunk_scale(const GradTable& t, int k, int chunk
 __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
     grad_scale_kernel(const __grid_constant__ GradTable t, const double* partial, int count, const float* norm_in,
                       float* norm_out, double max_norm) {
+  wait_for_previous();
   const double n = count ? total_norm(partial, count) : static_cast<double>(*norm_in);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(n);
   double ratio = max_norm / (n + 1e-6);
@@ -322,7 +325,7 @@ int launch_squares(const void* const* grads, const int64_t* sizes, const int* dt
     const int grid = grad_grid(t.first_chunk[t.count], d.sms);
     if (*parts + grid > workspace_doubles)
       return fail(SWIGLU_ERR_INVALID_ARGUMENT, "workspace of %lld doubles is too small", (long long)workspace_doubles);
-    grad_squares_kernel<<<grid, kGradThreads, 0, st>>>(t, workspace + *parts);
+    launch_after(grad_squares_kernel, grid, kGradThreads, 0, st, t, workspace + *parts);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "grad norm launch");
     *parts += grid;
@@ -338,8 +341,8 @@ int launch_scale(const void* const* grads, void* const* outs, const int64_t* siz
     GradTable t;
     k += fill_table(t, grads, outs, sizes, dtypes, k, count);
     if (t.count == 0) continue;
-    grad_scale_kernel<<<grad_grid(t.first_chunk[t.count], d.sms), kGradThreads, 0, st>>>(
-        t, partial, parts, norm_in, wrote ? nullptr : norm_out, max_norm);
+    launch_after(grad_scale_kernel, grad_grid(t.first_chunk[t.count], d.sms), kGradThreads, 0, st, t, partial, parts,
+                 norm_in, wrote ? nullptr : norm_out, max_norm);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "gradient scaling launch");
     wrote = true;
@@ -361,7 +364,7 @@ int op_grad_norm(const void* const* grads, const int64_t* sizes, const int* dtyp
   int parts = 0;
   if (int rc = launch_squares(grads, sizes, dtypes, count, workspace, workspace_doubles, *d, &parts, st)) return rc;
   if (parts == 0) return zero_norm(norm, st);
-  grad_norm_kernel<<<1, kGradThreads, 0, st>>>(workspace, parts, norm);
+  launch_after(grad_norm_kernel, 1, kGradThreads, 0, st, workspace, parts, norm);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "grad norm launch");
 }

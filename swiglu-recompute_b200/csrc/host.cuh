@@ -54,6 +54,24 @@ int check_mult8(const char* what, int64_t v);
 void choose_stream_k(int tiles, int clusters, int num_kb, long long tile_floats, int slabs, cudaStream_t st,
                      float** partials, uint32_t** counters, int* tail_out, int* split_out, uint32_t* epoch_out);
 
+// Launches a kernel that begins with wait_for_previous(): its blocks may be
+// placed while the stream's previous kernel drains (programmatic dependent
+// launch), which hides the 1-2 us between two kernels of a stream.
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
+}
+
 // Per-kernel launch state: dynamic shared memory opt-in done (bit per device)
 // and, for cluster kernels, how many CTA pairs fit at once on each device.
 struct KernelState {

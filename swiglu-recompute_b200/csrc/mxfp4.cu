@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) quantize_mxfp4_kernel(const 
                                                                           uint8_t* __restrict__ dst,
                                                                           uint8_t* __restrict__ scale, long long rows,
                                                                           int cols, int tiles_k) {
+  wait_for_previous();
   __shared__ __align__(16) uint8_t bytes[512];
   const QuantBlock q(cols, tiles_k);
   if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(bytes)[threadIdx.x] = 0;
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(kQuantThreads, 4) dequantize_mxfp4_kernel(cons
                                                                             const uint8_t* __restrict__ scale,
                                                                             T* __restrict__ dst, long long rows,
                                                                             int cols, int tiles_k) {
+  wait_for_previous();
   __shared__ __align__(16) uint8_t bytes[512];
   const QuantBlock q(cols, tiles_k);
   uint2 tile = make_uint2(0, 0);
@@ -270,14 +272,15 @@ int op_quantize(const void* src, void* dst, void* scale, int64_t rows, int64_t c
   DeviceInfo* d;
   if (int rc = current_device(&d)) return rc;
   const int tiles_k = static_cast<int>((cols + 127) / 128);
+  const auto to = static_cast<uint8_t*>(dst), scales = static_cast<uint8_t*>(scale);
+  const unsigned grid = quant_grid(rows, cols);
+  const int k = static_cast<int>(cols);
   if (dtype == SWIGLU_F32)
-    quantize_mxfp4_kernel<float><<<quant_grid(rows, cols), kQuantThreads, 0, st>>>(
-        static_cast<const float*>(src), static_cast<uint8_t*>(dst), static_cast<uint8_t*>(scale), rows,
-        static_cast<int>(cols), tiles_k);
+    launch_after(quantize_mxfp4_kernel<float>, grid, kQuantThreads, 0, st, static_cast<const float*>(src), to, scales,
+                 rows, k, tiles_k);
   else
-    quantize_mxfp4_kernel<__nv_bfloat16><<<quant_grid(rows, cols), kQuantThreads, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(src), static_cast<uint8_t*>(dst), static_cast<uint8_t*>(scale), rows,
-        static_cast<int>(cols), tiles_k);
+    launch_after(quantize_mxfp4_kernel<__nv_bfloat16>, grid, kQuantThreads, 0, st,
+                 static_cast<const __nv_bfloat16*>(src), to, scales, rows, k, tiles_k);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "quantize_mxfp4 launch");
 }
@@ -293,14 +296,15 @@ int op_dequantize(const void* q, const void* scale, void* dst, int64_t rows, int
   DeviceInfo* d;
   if (int rc = current_device(&d)) return rc;
   const int tiles_k = static_cast<int>((cols + 127) / 128);
+  const auto codes = static_cast<const uint8_t*>(q), scales = static_cast<const uint8_t*>(scale);
+  const unsigned grid = quant_grid(rows, cols);
+  const int k = static_cast<int>(cols);
   if (dtype == SWIGLU_F32)
-    dequantize_mxfp4_kernel<float><<<quant_grid(rows, cols), kQuantThreads, 0, st>>>(
-        static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), static_cast<float*>(dst), rows,
-        static_cast<int>(cols), tiles_k);
+    launch_after(dequantize_mxfp4_kernel<float>, grid, kQuantThreads, 0, st, codes, scales, static_cast<float*>(dst),
+                 rows, k, tiles_k);
   else
-    dequantize_mxfp4_kernel<__nv_bfloat16><<<quant_grid(rows, cols), kQuantThreads, 0, st>>>(
-        static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), static_cast<__nv_bfloat16*>(dst), rows,
-        static_cast<int>(cols), tiles_k);
+    launch_after(dequantize_mxfp4_kernel<__nv_bfloat16>, grid, kQuantThreads, 0, st, codes, scales,
+                 static_cast<__nv_bfloat16*>(dst), rows, k, tiles_k);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "dequantize_mxfp4 launch");
 }
@@ -375,6 +379,14 @@ int usable_sms(const DeviceInfo& d) {
   return sms < 2 ? 2 : sms;
 }
 
+// The second launch attribute of a cluster kernel that begins with
+// wait_for_previous().
+void after_previous(cudaLaunchAttribute* attr, cudaLaunchConfig_t& cfg) {
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
+}
+
 template <int NT, bool F32>
 int launch_cluster(const MxClusterParams& p, const MxPlan& plan, cudaStream_t st) {
   using Cfg = MxClusterCfg<NT, F32>;
@@ -387,9 +399,10 @@ int launch_cluster(const MxClusterParams& p, const MxPlan& plan, cudaStream_t st
     if (e != cudaSuccess) return cuda_fail(e, "matmul_mxfp4 launch");
     ks.ready.fetch_or(1ull << dev);
   }
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = pair_launch_config(attr, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, st);
   attr[0].val.clusterDim.x = plan.parts;
+  after_previous(attr, cfg);
   cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * p.tiles_x * plan.parts));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "matmul_mxfp4 launch");
@@ -408,8 +421,16 @@ int run_cluster(MxClusterParams& p, const MxPlan& plan, cudaStream_t st) {
 template <bool F32>
 int run_pair(MxParams& p, const DeviceInfo& d, cudaStream_t st) {
   using Cfg = MxCfg<F32>;
-  return launch_pair<mx_gemm_pair_kernel<Cfg>>(p, p.tiles_m * p.tiles_n, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, d, st,
-                                               "matmul_mxfp4 launch");
+  constexpr auto kern = mx_gemm_pair_kernel<Cfg>;
+  int cap = 0;
+  if (int rc = pair_capacity<kern>(Cfg::NUM_THREADS, Cfg::SMEM_BYTES, d, &cap, "matmul_mxfp4 launch")) return rc;
+  const int tiles = p.tiles_m * p.tiles_n;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = pair_launch_config(attr, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, st);
+  cfg.gridDim = dim3(2 * (tiles < cap ? tiles : cap));
+  after_previous(attr, cfg);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "matmul_mxfp4 launch");
 }
 
 int check_matmul(int64_t M, int64_t N, int64_t K) {

@@ -199,6 +199,7 @@ constexpr int kRowThreads = 1024;  // that a row may take, at 64 registers each
 
 template <typename T, typename W, bool E4M3, int VPT, bool SHIFT>
 __global__ void __launch_bounds__(kRowThreads) rmsnorm_fwd_row_kernel(const FwdParams p) {
+  wait_for_previous();
   constexpr int V = kV<T>;
   __shared__ float2 scratch[32];
   const long long row = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y;
@@ -277,6 +278,7 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_fwd_row_kernel(const FwdP
 // again from L1 / L2.
 template <typename T, typename W, bool E4M3>
 __global__ void __launch_bounds__(512) rmsnorm_fwd_any_kernel(const FwdParams p) {
+  wait_for_previous();
   __shared__ float2 scratch[16];
   const long long base = blockIdx.x * static_cast<long long>(p.cols);
   const T* x = static_cast<const T*>(p.x) + base;
@@ -344,6 +346,7 @@ constexpr int kBwdLoadRegs = 12 * VPT;
 template <typename T, typename W, int VPT, bool SHIFT>
 __global__ void __launch_bounds__(kBwdThreads, kBwdLoadRegs<VPT> <= 12 ? 2 : 1)
     rmsnorm_bwd_row_kernel(const BwdParams p) {
+  wait_for_previous();
   constexpr int V = kV<T>;
   __shared__ float2 scratch[2][32];
   __shared__ float parts[VPT == 1 ? 8 * 32 * V : 1];  // warp rows: [warp][pack element]
@@ -463,6 +466,7 @@ constexpr int kMaxStages = 8;
 
 template <typename T, typename W, int VPT>
 __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_ring_kernel(const BwdParams p) {
+  wait_for_previous();
   constexpr int V = kV<T>;
   extern __shared__ __align__(128) uint8_t ring[];  // [stage][dy, s, ds][cols]
   __shared__ uint64_t full[kMaxStages];
@@ -606,6 +610,7 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
 // block per row.
 template <typename T, typename W>
 __global__ void __launch_bounds__(512) rmsnorm_bwd_dot_kernel(const BwdParams p) {
+  wait_for_previous();
   __shared__ float2 scratch[16];
   const long long base = blockIdx.x * static_cast<long long>(p.cols);
   const T* dy = static_cast<const T*>(p.dy) + base;
@@ -620,6 +625,7 @@ __global__ void __launch_bounds__(512) rmsnorm_bwd_dot_kernel(const BwdParams p)
 // A thread per column walks a chunk of rows: dx, and its part of dweight.
 template <typename T, typename W>
 __global__ void __launch_bounds__(256) rmsnorm_bwd_cols_kernel(const BwdParams p) {
+  wait_for_previous();
   const int j = blockIdx.x * blockDim.x + threadIdx.x;
   if (j >= p.cols) return;
   const float w = to_f32(static_cast<const W*>(p.weight)[j]);
@@ -644,6 +650,7 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_cols_kernel(const BwdParams p
 // 32 threads along the chunks of each.
 template <typename W>
 __global__ void __launch_bounds__(1024) rmsnorm_dweight_kernel(const float* partial, W* dweight, int cols, int chunks) {
+  wait_for_previous();
   __shared__ float part[32][33];
   const int j = blockIdx.x * 32 + threadIdx.x;
   float acc = 0.0f;
@@ -683,7 +690,7 @@ bool launch_row(const FwdParams& p, cudaStream_t st) {
   const int x = threads_for(threads, kRowThreads);
   const dim3 block(x, x == 32 ? 4 : 1);
   const unsigned grid = static_cast<unsigned>((p.rows + block.y - 1) / block.y);
-  rmsnorm_fwd_row_kernel<T, W, E4M3, VPT, SHIFT><<<grid, block, 0, st>>>(p);
+  launch_after(rmsnorm_fwd_row_kernel<T, W, E4M3, VPT, SHIFT>, grid, block, 0, st, p);
   return true;
 }
 
@@ -708,7 +715,7 @@ int launch_fwd(const FwdParams& p, cudaStream_t st) {
   const bool done =
       grid16 && (whole ? launch_rows<T, W, E4M3, false>(p, st) : launch_rows<T, W, E4M3, true>(p, st));
   if (!done)
-    rmsnorm_fwd_any_kernel<T, W, E4M3><<<static_cast<unsigned>(p.rows), threads_for(p.cols, 512), 0, st>>>(p);
+    launch_after(rmsnorm_fwd_any_kernel<T, W, E4M3>, static_cast<unsigned>(p.rows), threads_for(p.cols, 512), 0, st, p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "rmsnorm forward launch");
 }
@@ -773,6 +780,8 @@ bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   const int64_t class_rows = (p.rows + p.period - 1) / p.period;
   const int64_t needed = (class_rows + block.y - 1) / block.y * p.period;
   p.chunks = static_cast<int>(grid > needed ? needed : grid);
+  // Not placed early: the blocks, fewer than fit an SM, would gather on the SMs
+  // that drain first (60000 x 512 bf16: 56 us against 78).
   rmsnorm_bwd_row_kernel<T, W, VPT, SHIFT><<<p.chunks, block, 0, st>>>(p);
   return true;
 }
@@ -802,7 +811,7 @@ bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 212 * 1024) != cudaSuccess) return false;
     ks.ready.fetch_or(1ull << dev);
   }
-  kern<<<p.chunks, x, p.stages * stage_bytes, st>>>(p);
+  launch_after(kern, p.chunks, x, p.stages * stage_bytes, st, p);
   return true;
 }
 
@@ -827,11 +836,11 @@ int launch_bwd(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
       grid16 && (whole ? launch_bwd_rows<T, W, false>(p, d, st) : launch_bwd_rows<T, W, true>(p, d, st));
   if (!done) p.chunks = chunks;
   if (!done) {
-    rmsnorm_bwd_dot_kernel<T, W><<<static_cast<unsigned>(p.rows), threads_for(p.cols, 512), 0, st>>>(p);
-    rmsnorm_bwd_cols_kernel<T, W><<<dim3((p.cols + 255) / 256, p.chunks), 256, 0, st>>>(p);
+    launch_after(rmsnorm_bwd_dot_kernel<T, W>, static_cast<unsigned>(p.rows), threads_for(p.cols, 512), 0, st, p);
+    launch_after(rmsnorm_bwd_cols_kernel<T, W>, dim3((p.cols + 255) / 256, p.chunks), 256, 0, st, p);
   }
-  rmsnorm_dweight_kernel<W><<<(p.cols + 31) / 32, dim3(32, 32), 0, st>>>(p.partial, static_cast<W*>(p.dweight), p.cols,
-                                                                         p.chunks);
+  launch_after(rmsnorm_dweight_kernel<W>, (p.cols + 31) / 32, dim3(32, 32), 0, st, p.partial,
+               static_cast<W*>(p.dweight), p.cols, p.chunks);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "rmsnorm backward launch");
 }

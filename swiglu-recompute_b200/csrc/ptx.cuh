@@ -41,6 +41,15 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 __device__ __forceinline__ uint32_t lane_id() { return threadIdx.x & 31u; }
 __device__ __forceinline__ uint32_t warp_id() { return threadIdx.x >> 5; }
 
+// First statement of a kernel launched with launch_after (host.cuh): lets the
+// next kernel's blocks take their places, then waits until the kernels before
+// this one are complete and their writes visible. Nothing may precede it (a
+// waiting block that already held TMEM could keep it from the kernel it waits
+// for).
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");

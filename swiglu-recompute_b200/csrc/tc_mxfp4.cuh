@@ -95,6 +95,7 @@ __device__ __forceinline__ void mx_store_chunk(const CUtensorMap* map, const uin
 
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const __grid_constant__ MxParams p) {
+  wait_for_previous();
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -363,6 +364,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::NUM_THREADS) mx_gemm_cluster_kernel(const __grid_constant__ MxClusterParams p) {
+  wait_for_previous();
   constexpr int STAGES = Cfg::STAGES, NT = Cfg::NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
