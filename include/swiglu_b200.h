@@ -352,6 +352,18 @@ int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, in
 int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
                              int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
 
+/* GEMM1 + SwiGLU with MXFP4 operands: preact [M, 2H] and h [M, H] (bf16, h from
+ * the rounded preact) from xq [M, K] and w1q [2H, K] (rows in `layout` order);
+ * the MXFP4 form of swiglu_b200_fused_matmul_swiglu_e4m3. K % 32 == 0,
+ * H % 128 == 0. One launch where the product takes pair tiles (the plan query,
+ * host-only, sets *fused to 1): preact or h may then be NULL. Elsewhere (few
+ * rows) the product is followed by swiglu_b200_forward_logic and preact must be
+ * given. */
+int swiglu_b200_fused_matmul_swiglu_mxfp4_plan(int64_t M, int64_t K, int64_t H, int num_sms, int* fused);
+int swiglu_b200_fused_matmul_swiglu_mxfp4(const void* xq, const void* x_scale, const void* w1q, const void* w1_scale,
+                                          void* preact, void* h, int64_t M, int64_t K, int64_t H, int layout,
+                                          void* stream);
+
 /* Whole forward of one MLP block: preact (saved for backward), h (caller's
  * transient workspace [M, H]) and y [M, Dout].
  * SwiGLUMemoryOptimizedFunction.forward (swiglu_recompute.py:59-66),

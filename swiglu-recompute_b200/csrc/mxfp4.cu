@@ -418,9 +418,8 @@ int run_cluster(MxClusterParams& p, const MxPlan& plan, cudaStream_t st) {
   }
 }
 
-template <bool F32>
+template <class Cfg>
 int run_pair(MxParams& p, const DeviceInfo& d, cudaStream_t st) {
-  using Cfg = MxCfg<F32>;
   constexpr auto kern = mx_gemm_pair_kernel<Cfg>;
   int cap = 0;
   if (int rc = pair_capacity<kern>(Cfg::NUM_THREADS, Cfg::SMEM_BYTES, d, &cap, "matmul_mxfp4 launch")) return rc;
@@ -478,7 +477,54 @@ int op_matmul(const void* aq, const void* a_scale, const void* bq, const void* b
   p.tiles_m = (int)((M + 255) / 256), p.tiles_n = (int)((N + 255) / 256);
   p.group_m = 16;
   p.status = d->status;
-  return f32 ? run_pair<true>(p, *d, st) : run_pair<false>(p, *d, st);
+  return f32 ? run_pair<MxCfg<true>>(p, *d, st) : run_pair<MxCfg<false>>(p, *d, st);
+}
+
+// Whether GEMM1 + SwiGLU runs as one launch: where its product takes pair tiles.
+bool swiglu_fused(int64_t M, int64_t K, int64_t H, int sms) { return plan_matmul(M, 2 * H, K, sms).pair; }
+
+int check_swiglu(int64_t M, int64_t K, int64_t H, int layout) {
+  if (int rc = check_dims("fused_matmul_swiglu_mxfp4", M, K, H)) return rc;
+  if (layout != SWIGLU_LAYOUT_STD && layout != SWIGLU_LAYOUT_PACKED128)
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "unknown layout %d", layout);
+  if (H <= 0 || H % 128)
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "H=%lld must be a positive multiple of 128", (long long)H);
+  return check_matmul(M, 2 * H, K);
+}
+
+int op_swiglu(const void* xq, const void* x_scale, const void* wq, const void* w_scale, void* preact, void* h,
+              int64_t M, int64_t K, int64_t H, int layout, cudaStream_t st) {
+  if (int rc = check_swiglu(M, K, H, layout)) return rc;
+  if (M == 0) return SWIGLU_OK;
+  if (!xq || !x_scale || !wq || !w_scale || (!preact && !h)) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned16(xq) || !aligned16(x_scale) || !aligned16(wq) || !aligned16(w_scale) || !aligned16(preact) ||
+      !aligned16(h))
+    return fail(SWIGLU_ERR_MISALIGNED, "fused_matmul_swiglu_mxfp4: pointers must be 16-byte aligned");
+  DeviceInfo* d;
+  if (int rc = current_device(&d)) return rc;
+  if (!swiglu_fused(M, K, H, usable_sms(*d))) {
+    if (!preact)
+      return fail(SWIGLU_ERR_INVALID_ARGUMENT, "fused_matmul_swiglu_mxfp4: this size needs preact (see the plan query)");
+    if (int rc = op_matmul(xq, x_scale, wq, w_scale, preact, M, 2 * H, K, SWIGLU_BF16, st)) return rc;
+    return h ? swiglu_b200_forward_logic(preact, h, M, H, SWIGLU_BF16, layout, st) : SWIGLU_OK;
+  }
+  MxParams p{};
+  if (int rc = make_map_bytes(&p.tmA, xq, K / 2, M, K / 2, 128, "x (MXFP4)")) return rc;
+  if (int rc = make_map_bytes(&p.tmB, wq, K / 2, 2 * H, K / 2, 128, "W1 (MXFP4)")) return rc;
+  if (int rc = make_map_scales(&p.tmAs, x_scale, M, K, "x scales")) return rc;
+  if (int rc = make_map_scales(&p.tmBs, w_scale, 2 * H, K, "W1 scales")) return rc;
+  if (preact) {
+    if (int rc = make_store_map(&p.tmC, preact, 2 * H, M, 2 * H, false)) return rc;
+  }
+  if (h) {
+    if (int rc = make_store_map(&p.tmD, h, H, M, H, false)) return rc;
+  }
+  p.M = (int)M, p.N = (int)(2 * H), p.K = (int)K, p.H = (int)H, p.layout = layout;
+  p.store_preact = preact != nullptr, p.store_h = h != nullptr;
+  p.tiles_m = (int)((M + 255) / 256), p.tiles_n = (int)(H / 128);
+  p.group_m = 16;
+  p.status = d->status;
+  return run_pair<MxCfg<false, true>>(p, *d, st);
 }
 
 }  // namespace
@@ -501,6 +547,21 @@ int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, in
 int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
                              int64_t M, int64_t N, int64_t K, int out_dtype, void* stream) {
   return op_matmul(aq, a_scale, bq, b_scale, c, M, N, K, out_dtype, static_cast<cudaStream_t>(stream));
+}
+
+int swiglu_b200_fused_matmul_swiglu_mxfp4_plan(int64_t M, int64_t K, int64_t H, int num_sms, int* fused) {
+  if (int rc = check_swiglu(M, K, H, SWIGLU_LAYOUT_STD)) return rc;
+  if (!fused) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
+  if (num_sms < 1) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "num_sms must be positive");
+  const int sms = num_sms - sm_reserve();
+  *fused = swiglu_fused(M, K, H, sms < 2 ? 2 : sms) ? 1 : 0;
+  return SWIGLU_OK;
+}
+
+int swiglu_b200_fused_matmul_swiglu_mxfp4(const void* xq, const void* x_scale, const void* w1q, const void* w1_scale,
+                                          void* preact, void* h, int64_t M, int64_t K, int64_t H, int layout,
+                                          void* stream) {
+  return op_swiglu(xq, x_scale, w1q, w1_scale, preact, h, M, K, H, layout, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -13,7 +13,9 @@
 //     stages or no stores: no change)
 //   whole warps, a lane elected for the instructions            485 us
 //     (without the copies 413, without waiting for a scale buffer 50 less)
-//   MXP_RESULT
+//   scales copied by a warp of their own, one commit for both CTAs  415-425 us
+//     (without the copies 373, one MMA of four 314, neither 306: operands
+//     from L2 at 16 TB/s)
 //
 // Out-of-range rows, columns of K and scale tiles are filled with zeros by TMA:
 // a zero code times 2^-127 is zero, so no tail needs a case of its own.
@@ -31,8 +33,11 @@ constexpr int kMxScaleBytes = 2 * kMxTileBytes;  // of 128 rows per stage
 struct MxParams {
   CUtensorMap tmA, tmB;    // codes, {128 bytes, 128 rows}
   CUtensorMap tmAs, tmBs;  // scale tiles as 32-bit cells, {256, 1}: both tiles of a stage
-  CUtensorMap tmC;         // output, {32 x 32} boxes
+  CUtensorMap tmC;         // output, {32 x 32} boxes (SwiGLU: preact)
+  CUtensorMap tmD;         // SwiGLU: h
   int M, N, K;
+  int H, layout;           // SwiGLU: N = 2 H columns in `layout` order, H % 128 == 0
+  bool store_preact, store_h;
   int tiles_m, tiles_n, group_m;
   uint32_t* status;
 };
@@ -42,9 +47,13 @@ struct MxParams {
 // ring, so that a stage's arrival also says that its scale buffer is free. The
 // epilogue reads the shared columns first and frees them, then the next tile's
 // MMAs may start: with two whole accumulators TMEM would be full.
-template <bool OUT_F32_>
+// SWIGLU: a tile is the left and the gate columns of 128 hidden units, rank 0
+// loading the left rows of B and rank 1 the gate rows, and the epilogue writes
+// preact and h = left * silu(gate) (fused_forward.py:101-185).
+template <bool OUT_F32_, bool SWIGLU_ = false>
 struct MxCfg {
   static constexpr bool OUT_F32 = OUT_F32_;
+  static constexpr bool SWIGLU = SWIGLU_;
   static constexpr int STAGES = 5;
   static constexpr int OPERAND_BYTES = 128 * 128;  // 128 rows
   static constexpr int SFA_OFFSET = 2 * OPERAND_BYTES;
@@ -55,7 +64,8 @@ struct MxCfg {
   static constexpr int NUM_THREADS = 224;
   static constexpr int BAR_BYTES = 8 * (3 * STAGES + 5) + 16;
   static constexpr int EPI_OFFSET = STAGES * STAGE_BYTES + ((BAR_BYTES + 1023) / 1024) * 1024;
-  static constexpr int SMEM_BYTES = 1024 + EPI_OFFSET + 4 * StoreStage<OUT_F32>::kWarpBytes;
+  static constexpr int EPI_WARP_BYTES = SWIGLU ? SwigluStage::kWarpBytes : StoreStage<OUT_F32>::kWarpBytes;
+  static constexpr int SMEM_BYTES = 1024 + EPI_OFFSET + 4 * EPI_WARP_BYTES;
   static_assert(SF_COL + 24 * STAGES <= 512, "TMEM holds 512 columns");
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
@@ -89,6 +99,47 @@ __device__ __forceinline__ void mx_store_chunk(const CUtensorMap* map, const uin
   __syncwarp();
   if (lane == 0) {
     tma_store_2d(map, buf, col, row0);
+    bulk_commit();
+  }
+}
+
+// One chunk of 32 hidden units of a SwiGLU tile: up to three {32 x 32} boxes
+// (preact left, preact gate, h) through one staging area, as
+// epilogue_swiglu_tma.
+__device__ __forceinline__ void mx_swiglu_chunk(const MxParams& p, const uint32_t (&rl)[32], const uint32_t (&rg)[32],
+                                                uint8_t* stage, int j, int row0) {
+  const uint32_t lane = threadIdx.x & 31u;
+  uint8_t* lbox = stage;
+  uint8_t* gbox = stage + SwigluStage::kBoxBytes;
+  uint8_t* hbox = stage + 2 * SwigluStage::kBoxBytes;
+  if (lane == 0) bulk_wait_read<0>();  // the previous chunk's stores have read the boxes
+  __syncwarp();
+  float v[32];
+  if (p.store_preact) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(rl[i]);
+    stage_row32_bf16(lbox, lane, v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(rg[i]);
+    stage_row32_bf16(gbox, lane, v);
+  }
+  if (p.store_h) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      // From the rounded preact, as the pointwise kernel of the other form.
+      const float l = bf16_round(__uint_as_float(rl[i])), g = bf16_round(__uint_as_float(rg[i]));
+      v[i] = l * (g * sigmoid_fast(g));
+    }
+    stage_row32_bf16(hbox, lane, v);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (p.store_preact) {
+      tma_store_2d(&p.tmC, lbox, left_col(j, p.H, p.layout), row0);
+      tma_store_2d(&p.tmC, gbox, gate_col(j, p.H, p.layout), row0);
+    }
+    if (p.store_h) tma_store_2d(&p.tmD, hbox, j, row0);
     bulk_commit();
   }
 }
@@ -148,8 +199,11 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
     for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
       int pm, pn;
       tile_coords(tile, p.tiles_m, p.tiles_n, p.group_m, pm, pn);
-      const int am = 2 * pm + static_cast<int>(rank);  // 128-row blocks of A and B of this CTA
-      const int bn = 2 * pn + static_cast<int>(rank);
+      const int am = 2 * pm + static_cast<int>(rank);  // 128-row tile of A of this CTA
+      // 128-row tiles of B: the two halves of every MMA's columns.
+      const int b0 = Cfg::SWIGLU ? left_col(pn * 128, p.H, p.layout) / 128 : 2 * pn;
+      const int b1 = Cfg::SWIGLU ? gate_col(pn * 128, p.H, p.layout) / 128 : 2 * pn + 1;
+      const int bn = leader ? b0 : b1;
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, status, kErrTimeoutProducer)) {
           ok = false;
@@ -163,8 +217,8 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
           tma_load_2d_pair(sa + Cfg::OPERAND_BYTES, &p.tmB, bar, kb * 128, bn * 128);
           tma_load_2d_pair(sa + Cfg::SFA_OFFSET, &p.tmAs, bar, kb * 256, am);
           // Every MMA reads the scales of all 256 columns in both CTAs.
-          tma_load_2d_pair(sa + Cfg::SFB_OFFSET, &p.tmBs, bar, kb * 256, 2 * pn);
-          tma_load_2d_pair(sa + Cfg::SFB_OFFSET + kMxScaleBytes, &p.tmBs, bar, kb * 256, 2 * pn + 1);
+          tma_load_2d_pair(sa + Cfg::SFB_OFFSET, &p.tmBs, bar, kb * 256, b0);
+          tma_load_2d_pair(sa + Cfg::SFB_OFFSET + kMxScaleBytes, &p.tmBs, bar, kb * 256, b1);
         }
         __syncwarp();
         filled |= 1u << stage;
@@ -269,7 +323,7 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
   } else {
     const uint32_t q = warp & 3u;
     uint32_t acc = 0, acc_phase = 0;
-    uint8_t* stage = smem + Cfg::EPI_OFFSET + (warp - 2) * StoreStage<Cfg::OUT_F32>::kWarpBytes;
+    uint8_t* stage = smem + Cfg::EPI_OFFSET + (warp - 2) * Cfg::EPI_WARP_BYTES;
     constexpr int kBufBytes = StoreStage<Cfg::OUT_F32>::kWarpBytes / 2;
     for (int tile = first_tile; tile < tiles; tile += tile_step) {
       int pm, pn;
@@ -278,26 +332,47 @@ __global__ void __launch_bounds__(Cfg::NUM_THREADS, 1) mx_gemm_pair_kernel(const
       tc_fence_after_sync();
       const int row0 = pm * 256 + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * Cfg::ACC_STEP;
-      // Shared columns first: chunks 7..4 of accumulator 0, 0..3 of accumulator 1.
-      const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
       uint32_t r[4][32];
+      auto free_shared = [&] {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_rank(tmem_free, 0));
+      };
+      if constexpr (Cfg::SWIGLU) {
+        // The shared columns are the gate half of accumulator 0 and the left half of
+        // accumulator 1: one half is read and freed, the other follows chunk by chunk.
+        const int half = acc == 0 ? 128 : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + i * c_step) * 32, r[i]);
-      tmem_ld_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_rank(tmem_free, 0));
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + half + i * 32, r[i]);
+        tmem_ld_wait();
+        free_shared();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
-                                     pn * 256 + (c_first + i * c_step) * 32, row0);
+        for (int i = 0; i < 4; ++i) {
+          uint32_t other[32];
+          tmem_ld_32x32b_x32(t_row + (128 - half) + i * 32, other);
+          tmem_ld_wait();
+          if (acc == 0) mx_swiglu_chunk(p, other, r[i], stage, pn * 128 + i * 32, row0);
+          else mx_swiglu_chunk(p, r[i], other, stage, pn * 128 + i * 32, row0);
+        }
+      } else {
+        // Shared columns first: chunks 7..4 of accumulator 0, 0..3 of accumulator 1.
+        const int c_first = acc == 0 ? 7 : 0, c_step = acc == 0 ? -1 : 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + (4 + i) * c_step) * 32, r[i]);
-      tmem_ld_wait();
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + i * c_step) * 32, r[i]);
+        tmem_ld_wait();
+        free_shared();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
-                                     pn * 256 + (c_first + (4 + i) * c_step) * 32, row0);
+        for (int i = 0; i < 4; ++i)
+          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
+                                       pn * 256 + (c_first + i * c_step) * 32, row0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_row + (c_first + (4 + i) * c_step) * 32, r[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mx_store_chunk<Cfg::OUT_F32>(&p.tmC, r[i], stage + (i & 1) * kBufBytes,
+                                       pn * 256 + (c_first + (4 + i) * c_step) * 32, row0);
+      }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }

@@ -63,6 +63,8 @@ _SIGNATURES = {
     "swiglu_b200_quantize_mxfp4": [_p, _p, _p, _i64, _i64, _i, _p],
     "swiglu_b200_dequantize_mxfp4": [_p, _p, _p, _i64, _i64, _i, _p],
     "swiglu_b200_matmul_mxfp4": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p],
+    "swiglu_b200_fused_matmul_swiglu_mxfp4_plan": [_i64, _i64, _i64, _i, ctypes.POINTER(_i)],
+    "swiglu_b200_fused_matmul_swiglu_mxfp4": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p],
     "swiglu_b200_mlp_forward":
         [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _p],
     "swiglu_b200_mlp_backward":

@@ -187,6 +187,31 @@ def _(aq, a_scale, bq, b_scale):
     return aq.new_empty((aq.shape[0], bq.shape[0]), dtype=torch.bfloat16)
 
 
+@torch.library.custom_op(f"{_NS}::swiglu_fwd_mxfp4", mutates_args=(), device_types="cuda")
+def swiglu_fwd_mxfp4(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+                     layout: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(preact [M, 2H], h [M, H]) in bf16 from MXFP4 x and W1 rows."""
+    return ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=layout)
+
+
+@swiglu_fwd_mxfp4.register_fake
+def _(xq, xs, wq, ws, layout):
+    m, n2 = xq.shape[0], wq.shape[0]
+    return (xq.new_empty((m, n2), dtype=torch.bfloat16), xq.new_empty((m, n2 // 2), dtype=torch.bfloat16))
+
+
+@torch.library.custom_op(f"{_NS}::swiglu_fwd_mxfp4_h", mutates_args=(), device_types="cuda")
+def swiglu_fwd_mxfp4_h(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+                       layout: int) -> torch.Tensor:
+    """h [M, H] only (the no-save MXFP4 forward)."""
+    return ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=layout, want_preact=False)[1]
+
+
+@swiglu_fwd_mxfp4_h.register_fake
+def _(xq, xs, wq, ws, layout):
+    return xq.new_empty((xq.shape[0], wq.shape[0] // 2), dtype=torch.bfloat16)
+
+
 # Without a residual the stream is x itself, which an op may not return: its
 # place holds an empty tensor then.
 @torch.library.custom_op(f"{_NS}::rmsnorm_fwd", mutates_args=(), device_types="cuda")
@@ -289,6 +314,14 @@ class _Eager:
         return ops.matmul_mxfp4(aq, a_scale, bq, b_scale)
 
     @staticmethod
+    def swiglu_fwd_mxfp4(xq, xs, wq, ws, layout):
+        return ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=layout)
+
+    @staticmethod
+    def swiglu_fwd_mxfp4_h(xq, xs, wq, ws, layout):
+        return ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=layout, want_preact=False)[1]
+
+    @staticmethod
     def rmsnorm_fwd(x, weight, residual, eps):
         return ops.rmsnorm_fwd(x, weight, residual, eps=eps)
 
@@ -355,6 +388,14 @@ class _Traced:
     @staticmethod
     def matmul_mxfp4(aq, a_scale, bq, b_scale):
         return torch.ops.swiglu_b200.matmul_mxfp4(aq, a_scale, bq, b_scale)
+
+    @staticmethod
+    def swiglu_fwd_mxfp4(xq, xs, wq, ws, layout):
+        return torch.ops.swiglu_b200.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout)
+
+    @staticmethod
+    def swiglu_fwd_mxfp4_h(xq, xs, wq, ws, layout):
+        return torch.ops.swiglu_b200.swiglu_fwd_mxfp4_h(xq, xs, wq, ws, layout)
 
     @staticmethod
     def rmsnorm_fwd(x, weight, residual, eps):

@@ -613,3 +613,26 @@ def matmul_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_sc
     _launch(dev, "swiglu_b200_matmul_mxfp4", aq.data_ptr(), a_scale.data_ptr(), bq.data_ptr(), b_scale.data_ptr(),
             out.data_ptr(), M, N, K, dt)
     return out
+
+
+def swiglu_fwd_mxfp4(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, *, layout: int,
+                     want_h: bool = True, want_preact: bool = True):
+    """(preact [M, 2H] or None, h [M, H] or None) in bf16 from MXFP4 x [M, K]
+    and W1 [2H, K] (rows in `layout` order); h from the rounded preact.
+    H % 128 == 0."""
+    assert want_h or want_preact
+    dev = _check_cuda(xq, x_scale, wq, w_scale)
+    M, K = _check_mx(xq, x_scale)
+    n2, K2 = _check_mx(wq, w_scale)
+    if K != K2 or n2 % 256:
+        raise ValueError(f"x [{M}, {K}] and W1 [{n2}, {K2}]: inner dimensions must agree and H be a multiple of 128")
+    H = n2 // 2
+    # Few rows take two launches, with preact between them.
+    fused = ctypes.c_int(0)
+    if not want_preact:
+        _lib.call("swiglu_b200_fused_matmul_swiglu_mxfp4_plan", M, K, H, _num_sms(dev.index), ctypes.byref(fused))
+    preact = None if fused.value else xq.new_empty((M, n2), dtype=torch.bfloat16)
+    h = xq.new_empty((M, H), dtype=torch.bfloat16) if want_h else None
+    _launch(dev, "swiglu_b200_fused_matmul_swiglu_mxfp4", xq.data_ptr(), x_scale.data_ptr(), wq.data_ptr(),
+            w_scale.data_ptr(), _ptr(preact), _ptr(h), M, K, H, layout)
+    return preact if want_preact else None, h

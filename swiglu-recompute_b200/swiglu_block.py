@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 from swiglu_b200 import ops
 from swiglu_b200.library import kernels
 from swiglu_b200.ops import LAYOUT_STD, W1_ROWS
-from swiglu_recompute import _flatten_rows, _recompute_backward
+from swiglu_recompute import _flatten_rows, _mxfp4_gemm1, _recompute_backward
 
 PRECISIONS = ("bf16", "e4m3", "mxfp4")
 
@@ -94,9 +94,9 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
         else:
             n, s, rstd = K.rmsnorm_fwd(x2, g, r2, eps)
             if precision == "mxfp4":
-                preact = K.matmul_mxfp4(*K.quantize_mxfp4(n), *K.quantize_mxfp4(W1c))
+                nq, ns = K.quantize_mxfp4(n)
                 del n
-                h = K.forward_logic(preact, LAYOUT_STD)
+                preact, h = _mxfp4_gemm1(K, nq, ns, *K.quantize_mxfp4(W1c), training)
                 y = K.matmul_mxfp4(*K.quantize_mxfp4(h), *K.quantize_mxfp4(W2c))
             else:
                 if training:

@@ -228,11 +228,23 @@ class SwiGLUFP8ForwardFunction(torch.autograd.Function):
         return gx, gw1, gw2
 
 
+def _mxfp4_gemm1(K, xq, xs, w1q, w1s, save_preact):
+    """(preact or None, h) of GEMM1 + SwiGLU with MXFP4 operands: the fused form
+    where H is a multiple of 128 (whole scale tiles in both halves of W1), else
+    the product and the pointwise kernel."""
+    if w1q.shape[0] % 256 == 0:
+        if save_preact:
+            return K.swiglu_fwd_mxfp4(xq, xs, w1q, w1s, LAYOUT_STD)
+        return None, K.swiglu_fwd_mxfp4_h(xq, xs, w1q, w1s, LAYOUT_STD)
+    preact = K.matmul_mxfp4(xq, xs, w1q, w1s)
+    return preact, K.forward_logic(preact, LAYOUT_STD)
+
+
 class SwiGLUFP4ForwardFunction(torch.autograd.Function):
     """Forward GEMMs with MXFP4 operands, backward as the recompute Function.
 
     x, W1, h and W2 are quantised in blocks of 32 along the contraction (e2m1
-    codes, one power-of-two scale a block); preact = x W1^T and y = h W2^T run
+    codes, one power-of-two scale a block); GEMM1 + SwiGLU and y = h W2^T run
     on the tensor core's block-scaled 4-bit kind with f32 accumulation. preact
     (bf16) is saved as in SwiGLUMemoryOptimizedFunction, whose bf16 backward
     follows unchanged. No counterpart in the reference; results differ from the
@@ -245,14 +257,13 @@ class SwiGLUFP4ForwardFunction(torch.autograd.Function):
         x2 = _flatten_rows(x)
         W1c, W2c = W1.contiguous(), W2.contiguous()
         K = kernels()
-        xq, xs = K.quantize_mxfp4(x2)
-        w1q, w1s = K.quantize_mxfp4(W1c)
-        preact = K.matmul_mxfp4(xq, xs, w1q, w1s)
-        del xq, w1q
-        hq, hs = K.quantize_mxfp4(K.forward_logic(preact, LAYOUT_STD))
+        training = any(ctx.needs_input_grad[:3])
+        preact, h = _mxfp4_gemm1(K, *K.quantize_mxfp4(x2), *K.quantize_mxfp4(W1c), training)
+        hq, hs = K.quantize_mxfp4(h)
+        del h
         w2q, w2s = K.quantize_mxfp4(W2c)
         y = K.matmul_mxfp4(hq, hs, w2q, w2s)
-        if any(ctx.needs_input_grad[:3]):
+        if training:
             ctx.save_for_backward(x2, W1c, W2c, preact)
         ctx.x_shape = x.shape
         return y.reshape(*lead, W2.shape[0])
@@ -336,8 +347,8 @@ class SwiGLUMLPFP4Inference(nn.Module):
         if x.dtype != torch.bfloat16:
             raise TypeError("the MXFP4 forward takes bf16 activations")
         K = kernels()
-        preact = K.matmul_mxfp4(*K.quantize_mxfp4(_flatten_rows(x)), self.w1_q, self.w1_scale)
-        y = K.matmul_mxfp4(*K.quantize_mxfp4(K.forward_logic(preact, LAYOUT_STD)), self.w2_q, self.w2_scale)
+        _, h = _mxfp4_gemm1(K, *K.quantize_mxfp4(_flatten_rows(x)), self.w1_q, self.w1_scale, False)
+        y = K.matmul_mxfp4(*K.quantize_mxfp4(h), self.w2_q, self.w2_scale)
         return y.reshape(*x.shape[:-1], y.shape[-1])
 
 

@@ -66,7 +66,8 @@ def test_fp4_forward_traces(traced):
 
     t = _targets(make_fx(f, tracing_mode="fake")(*args))
     assert sum(x == "swiglu_b200.quantize_mxfp4.default" for x in t) == 4
-    assert sum(x == "swiglu_b200.matmul_mxfp4.default" for x in t) == 2
+    assert sum(x == "swiglu_b200.matmul_mxfp4.default" for x in t) == 1
+    assert sum(x == "swiglu_b200.swiglu_fwd_mxfp4.default" for x in t) == 1
 
 
 def test_refusals():
@@ -83,7 +84,8 @@ def test_refusals():
     with pytest.raises(ValueError, match="CUDA"):   # no CPU path
         b(x, x)
     assert SB.clip_grad_norm_(b.parameters(), 1.0) == 0   # no gradients yet
-    for name in ("forward_logic", "quantize_mxfp4", "matmul_mxfp4", "rmsnorm_fwd", "rmsnorm_fwd_e4m3", "rmsnorm_bwd"):
+    for name in ("forward_logic", "quantize_mxfp4", "matmul_mxfp4", "rmsnorm_fwd", "rmsnorm_fwd_e4m3", "rmsnorm_bwd",
+                 "swiglu_fwd_mxfp4", "swiglu_fwd_mxfp4_h"):
         s = getattr(torch.ops.swiglu_b200, name).default._schema
         assert not any(a.alias_info is not None and a.alias_info.is_write for a in s.arguments), name
 

@@ -30,6 +30,13 @@ def _bf(t):
     return t.to(BF).double()
 
 
+def _mx_gemm1(x, w1):
+    if w1.shape[0] % 256 == 0:
+        return ops.swiglu_fwd_mxfp4(*ops.quantize_mxfp4(x), *ops.quantize_mxfp4(w1), layout=ops.LAYOUT_STD)
+    pre = ops.matmul_mxfp4(*ops.quantize_mxfp4(x), *ops.quantize_mxfp4(w1))
+    return pre, ops.forward_logic(pre, layout=ops.LAYOUT_STD)
+
+
 def _chain(x, r, g, w1, w2, precision, eps=1e-6):
     """(y, s, preact) by the operators one after another, on the device."""
     if precision == "e4m3":
@@ -38,8 +45,7 @@ def _chain(x, r, g, w1, w2, precision, eps=1e-6):
         return ops.matmul_e4m3(*ops.quantize_rows_e4m3(h), *ops.quantize_rows_e4m3(w2)), s, pre
     n, s, _ = ops.rmsnorm_fwd(x, g, r, eps=eps)
     if precision == "mxfp4":
-        pre = ops.matmul_mxfp4(*ops.quantize_mxfp4(n), *ops.quantize_mxfp4(w1))
-        h = ops.forward_logic(pre, layout=ops.LAYOUT_STD)
+        pre, h = _mx_gemm1(n, w1)
         return ops.matmul_mxfp4(*ops.quantize_mxfp4(h), *ops.quantize_mxfp4(w2)), s, pre
     pre, h = ops.swiglu_fwd(n, w1, w_form=ops.W1_ROWS, layout=ops.LAYOUT_STD, h_from_rounded=True)
     return ops.matmul(h, w2, a_t=False, b_t=True), s, pre
@@ -175,7 +181,8 @@ def test_norm_module():
         n(xd, rd.float())
 
 
-@pytest.mark.parametrize("M,D,H,Dout", [(1, 256, 512, 256), (5, 512, 256, 128), (384, 256, 384, 264)])
+@pytest.mark.parametrize("M,D,H,Dout", [(1, 256, 512, 256), (5, 512, 256, 128), (384, 256, 384, 264),
+                                        (200, 96, 160, 64)])
 def test_fp4_modules(M, D, H, Dout):
     x, w1, w2, gy = O.make_inputs(M, D, H, Dout, seed=6, dtype=BF)
     m = SR.SwiGLUMLPFP4Forward(D, H, Dout, dtype=BF).to(DEV)
@@ -185,8 +192,7 @@ def test_fp4_modules(M, D, H, Dout):
     xd = x.to(DEV).requires_grad_(True)
     y = m(xd)
     with torch.no_grad():
-        pre = ops.matmul_mxfp4(*ops.quantize_mxfp4(x.to(DEV)), *ops.quantize_mxfp4(m.w1))
-        h = ops.forward_logic(pre, layout=ops.LAYOUT_STD)
+        pre, h = _mx_gemm1(x.to(DEV), m.w1)
         assert torch.equal(y, ops.matmul_mxfp4(*ops.quantize_mxfp4(h), *ops.quantize_mxfp4(m.w2)))
     gx, gw1, gw2 = torch.autograd.grad(y, [xd, m.w1, m.w2], gy.to(DEV))
     left, gate = pre.double().cpu().chunk(2, 1)

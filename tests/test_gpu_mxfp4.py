@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from oracle import operators as O
+from oracle import swiglu_oracle as SO
 from swiglu_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -93,6 +94,38 @@ def _check(c, av, bv, out):
 @pytest.mark.parametrize("out", [BF, F32])
 def test_product(M, N, K, out):
     _check(*_product(M, N, K, out), out)
+
+
+@pytest.mark.parametrize("layout", [SO.STD, SO.PACKED])
+@pytest.mark.parametrize("M,K,H", [(1, 256, 128), (17, 1056, 384), (100, 512, 256), (257, 64, 128), (300, 1440, 640),
+                                   (1500, 512, 1408), (4100, 96, 256)])
+def test_swiglu_forward(layout, M, K, H):
+    """preact as the product gives it (its own tests hold that to f64), h within
+    one bf16 rounding of left * silu(gate) of that preact, and the same bits
+    whichever outputs are asked for."""
+    lay = ops.LAYOUT_STD if layout == SO.STD else ops.LAYOUT_PACKED128
+    x, w1 = _matrix(M, K, BF), (_matrix(2 * H, K, BF, 1) * K ** -0.5).to(BF)
+    li, gi = SO.col_index(H, layout)
+    w = torch.empty_like(w1)
+    w[li], w[gi] = w1[:H], w1[H:]
+    xq, xs = ops.quantize_mxfp4(x.to(DEV))
+    wq, ws = ops.quantize_mxfp4(w.to(DEV))
+    preact, h = ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=lay)
+    assert torch.equal(preact, ops.matmul_mxfp4(xq, xs, wq, ws))
+    p = preact.double().cpu()
+    left, gate = p[:, li], p[:, gi]
+    ref = left * gate * torch.sigmoid(gate)
+    # Half a bf16 step, and the f32 sigmoid 1 / (1 + e^-g) of the fused form. By the
+    # CUDA programming guide's table __expf(x) is off by at most 2 + 1.173 |x| ulp and
+    # __fdividef by 2, and __fdividef gives 0 for a divisor above 2^126: with the three
+    # other roundings (1 + e, g s, l silu) at most 7 + 1.173 |g| ulp of 2^-23, and below
+    # g = -87 an absolute |l g| 2^-126. (The pointwise kernel's expf and division are
+    # within 2 ulp each.) The gates here reach hundreds.
+    bound = (2 ** -8 + (7 + 1.173 * gate.abs()) * 2.0 ** -23) * ref.abs() + (left * gate).abs() * 2.0 ** -126 + 1e-37
+    assert torch.all((h.double().cpu() - ref).abs() <= bound)
+    assert torch.equal(ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=lay, want_preact=False)[1], h)
+    assert torch.equal(ops.swiglu_fwd_mxfp4(xq, xs, wq, ws, layout=lay, want_h=False)[0], preact)
+    assert ops.device_status(0) == 0
 
 
 @pytest.mark.parametrize("M", [1, 5, 40, 130, 600])

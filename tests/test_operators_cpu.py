@@ -100,6 +100,20 @@ def test_mxfp4_refusals(lib):
     assert m(None, None, None, None, None, 0, 8, 64, 1, None) == 0
 
 
+def test_mxfp4_swiglu_refusals_and_plan(lib):
+    f, plan = lib.swiglu_b200_fused_matmul_swiglu_mxfp4, lib.swiglu_b200_fused_matmul_swiglu_mxfp4_plan
+    _said(lib, f(P, P, P, P, P, P, 4, 64, 96, 0, None), 1, b"multiple of 128")
+    _said(lib, f(P, P, P, P, P, P, 4, 40, 128, 0, None), 1, b"multiple of 32")
+    _said(lib, f(P, P, P, P, P, P, 4, 64, 128, 2, None), 1, b"layout")
+    _said(lib, f(P, P, P, P, None, None, 4, 64, 128, 0, None), 1, b"null")
+    _said(lib, f(P, P, P, P, P, P + 2, 4, 64, 128, 0, None), 2, b"16-byte")
+    assert f(None, None, None, None, None, None, 0, 64, 128, 0, None) == 0
+    fused = ctypes.c_int(-1)
+    for M, K, H, want in [(11136, 3584, 14336, 1), (1, 3584, 14336, 0), (64, 1024, 2816, 0), (4096, 1024, 2816, 1)]:
+        assert plan(M, K, H, 148, ctypes.byref(fused)) == 0 and fused.value == want, (M, K, H)
+    _said(lib, plan(4, 64, 128, 0, ctypes.byref(fused)), 1, b"num_sms")
+
+
 def test_python_refusals_without_a_device():
     t = torch.ones(4, 64)
     for call in (lambda: ops.rmsnorm_fwd(t, t[0]), lambda: ops.quantize_mxfp4(t), lambda: ops.grad_norm([t]),
