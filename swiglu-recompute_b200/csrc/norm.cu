@@ -69,6 +69,17 @@ __device__ __forceinline__ uint4 set16(const float (&f)[kV<T>]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
 }
 
+template <typename T>
+__device__ __forceinline__ uint4 unpairs16(const float2 (&f)[kV<T> / 2]) {
+  float v[kV<T>];
+#pragma unroll
+  for (int i = 0; i < kV<T> / 2; ++i) {
+    v[2 * i] = f[i].x;
+    v[2 * i + 1] = f[i].y;
+  }
+  return set16<T>(v);
+}
+
 // Rows whose length is no multiple of a pack (SHIFT): the packs stay on the
 // tensor's 16-byte grid, so a row starts `head` elements inside its first one.
 // Pack k holds the row's elements k * V - head and on; in the first and the last
@@ -219,34 +230,41 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_fwd_row_kernel(const FwdP
       if (k < rp.packs) b[i] = rp.load(static_cast<const T*>(p.residual), k);
     }
   }
-  float sum = 0.0f, top = 0.0f;
+  // The kernel comes close to issuing an instruction every cycle (75 % of the slots
+  // for bf16 in scalar form), hence the packed f32x2 arithmetic.
+  constexpr int P = V / 2;
+  float2 sum2 = make_float2(0.0f, 0.0f);
+  float top = 0.0f;
   float sw[E4M3 ? VPT : 1][V];  // s w, kept for the e4m3 output
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
     if (k >= rp.packs) continue;
-    float v[V];
-    get16<T>(a[i], v);
+    float2 v[P];
+    pairs16<T>(a[i], v);
     if (p.residual) {
-      float r[V];
-      get16<T>(b[i], r);
+      float2 r[P];
+      pairs16<T>(b[i], r);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] += r[e];
-      a[i] = set16<T>(v);
+      for (int e = 0; e < P; ++e) v[e] = __fadd2_rn(v[e], r[e]);
+      a[i] = unpairs16<T>(v);
       rp.store(static_cast<T*>(p.s), k, a[i]);
-      get16<T>(a[i], v);
+      pairs16<T>(a[i], v);
     }
     if constexpr (E4M3) {
       rp.weight(w, k, sw[i]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        sw[i][e] *= v[e];
-        top = fmaxf(top, fabsf(sw[i][e]));
+      for (int e = 0; e < P; ++e) {
+        const float2 m = __fmul2_rn(make_float2(sw[i][2 * e], sw[i][2 * e + 1]), v[e]);
+        sw[i][2 * e] = m.x;
+        sw[i][2 * e + 1] = m.y;
+        top = fmaxf(top, fmaxf(fabsf(m.x), fabsf(m.y)));
       }
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum += v[e] * v[e];
+    for (int e = 0; e < P; ++e) sum2 = __ffma2_rn(v[e], v[e], sum2);
   }
+  float sum = sum2.x + sum2.y;
   row_reduce(sum, top, blockDim.x >> 5, scratch);
   float rstd, qs, scale;
   row_factors(sum, top, p, rstd, qs, scale);
@@ -260,15 +278,21 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_fwd_row_kernel(const FwdP
     if (k >= rp.packs) continue;
     if constexpr (E4M3) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) sw[i][e] *= qs;
+      for (int e = 0; e < P; ++e) {
+        const float2 m = __fmul2_rn(make_float2(sw[i][2 * e], sw[i][2 * e + 1]), make_float2(qs, qs));
+        sw[i][2 * e] = m.x;
+        sw[i][2 * e + 1] = m.y;
+      }
       rp.store_e4m3(static_cast<uint8_t*>(p.y), k, sw[i]);
     } else {
-      float v[V], f[V];
-      get16<T>(a[i], v);
+      float2 v[P];
+      float f[V];
+      pairs16<T>(a[i], v);
       rp.weight(w, k, f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] *= rstd * f[e];
-      rp.store(static_cast<T*>(p.y), k, set16<T>(v));
+      for (int e = 0; e < P; ++e)
+        v[e] = __fmul2_rn(__fmul2_rn(v[e], make_float2(rstd, rstd)), make_float2(f[2 * e], f[2 * e + 1]));
+      rp.store(static_cast<T*>(p.y), k, unpairs16<T>(v));
     }
   }
 }
@@ -571,13 +595,7 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
         d[e] = __ffma2_rn(v[m][e], c2, d[e]);
         d[e] = __ffma2_rn(__fmul2_rn(g[m][e], rstd2), w[i][e], d[e]);
       }
-      float f[V];
-#pragma unroll
-      for (int e = 0; e < P; ++e) {
-        f[2 * e] = d[e].x;
-        f[2 * e + 1] = d[e].y;
-      }
-      out[k] = set16<T>(f);
+      out[k] = unpairs16<T>(d);
     }
     if (++stage == p.stages) {
       stage = 0;
@@ -646,25 +664,41 @@ __global__ void __launch_bounds__(256) rmsnorm_bwd_cols_kernel(const BwdParams p
   p.partial[blockIdx.y * static_cast<long long>(p.cols) + j] = acc;
 }
 
-// dweight = sum of the chunks' parts, in a fixed order: 32 columns a block,
-// 32 threads along the chunks of each.
+// dweight = sum of the chunks' parts, in a fixed order: 32 columns a block, 128
+// threads along the chunks for each four of them, so that a thread's few loads
+// are all in flight at once (with 32 threads along the chunks the sum of 296
+// parts of 3584 columns took 7 us).
 template <typename W>
 __global__ void __launch_bounds__(1024) rmsnorm_dweight_kernel(const float* partial, W* dweight, int cols, int chunks) {
   wait_for_previous();
-  __shared__ float part[32][33];
-  const int j = blockIdx.x * 32 + threadIdx.x;
-  float acc = 0.0f;
+  __shared__ float part[128][33];
+  const int tx = static_cast<int>(threadIdx.x & 7), ty = static_cast<int>(threadIdx.x >> 3);
+  const int j = blockIdx.x * 32 + tx * 4;
+  float acc[4] = {};
   if (j < cols) {
+    const bool whole = cols % 4 == 0;  // every part's row then starts on the 16-byte grid
 #pragma unroll 4
-    for (int c = threadIdx.y; c < chunks; c += 32) acc += partial[c * static_cast<long long>(cols) + j];
-  }
-  part[threadIdx.y][threadIdx.x] = acc;
-  __syncthreads();
-  acc = part[threadIdx.x][threadIdx.y];
+    for (int c = ty; c < chunks; c += 128) {
+      const float* p = partial + c * static_cast<long long>(cols) + j;
+      if (whole) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
+      } else {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  const int k = blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && k < cols) dweight[k] = from_f32<W>(acc);
+        for (int i = 0; i < 4; ++i)
+          if (j + i < cols) acc[i] += p[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[ty][tx * 4 + i] = acc[i];
+  __syncthreads();
+  const int lane = static_cast<int>(lane_id()), k = static_cast<int>(warp_id());
+  float sum = (part[lane][k] + part[lane + 32][k]) + (part[lane + 64][k] + part[lane + 96][k]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int col = blockIdx.x * 32 + k;
+  if (lane == 0 && col < cols) dweight[col] = from_f32<W>(sum);
 }
 
 int check_norm(const char* what, int64_t rows, int64_t cols, int dtype, int weight_dtype) {
@@ -786,7 +820,8 @@ bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   return true;
 }
 
-// Rows of 128 packs or more, at least two of them in the ring: 210 KB of shared memory an SM over the blocks its registers hold.
+// Rows of 128 packs or more, at least two of them in the ring: 210 KB of shared
+// memory an SM over the blocks its registers hold.
 template <typename T, typename W, int VPT>
 bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   const int64_t threads = (p.cols / kV<T> + VPT - 1) / VPT;
@@ -839,20 +874,21 @@ int launch_bwd(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
     launch_after(rmsnorm_bwd_dot_kernel<T, W>, static_cast<unsigned>(p.rows), threads_for(p.cols, 512), 0, st, p);
     launch_after(rmsnorm_bwd_cols_kernel<T, W>, dim3((p.cols + 255) / 256, p.chunks), 256, 0, st, p);
   }
-  launch_after(rmsnorm_dweight_kernel<W>, (p.cols + 31) / 32, dim3(32, 32), 0, st, p.partial,
+  launch_after(rmsnorm_dweight_kernel<W>, (p.cols + 31) / 32, 1024, 0, st, p.partial,
                static_cast<W*>(p.dweight), p.cols, p.chunks);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SWIGLU_OK : cuda_fail(e, "rmsnorm backward launch");
 }
 
-// Floats of the workspace: the rows' dots, then the parts of dweight of
-// whichever kernels run.
+// Floats of the workspace: the rows' dots (a multiple of four), then the parts of
+// dweight of whichever kernels run.
+int64_t dot_floats(int64_t rows) { return (rows + 3) / 4 * 4; }
 int64_t bwd_floats(int64_t rows, int64_t cols, int sms) {
   if (rows == 0) return 0;
   int chunks, per;
   plan_bwd(rows, cols, sms, &chunks, &per);
   const int64_t blocks = most_bwd_blocks(rows, cols, sms);
-  return rows + (blocks > chunks ? blocks : chunks) * cols;
+  return dot_floats(rows) + (blocks > chunks ? blocks : chunks) * cols;
 }
 
 int op_rmsnorm_bwd(BwdParams p, int64_t rows, int64_t cols, int dtype, int weight_dtype, float* workspace,
@@ -880,7 +916,7 @@ int op_rmsnorm_bwd(BwdParams p, int64_t rows, int64_t cols, int dtype, int weigh
                 (long long)workspace_floats, (long long)bwd_floats(rows, cols, d->sms));
   p.status = d->status;
   p.dot = workspace;
-  p.partial = workspace + rows;
+  p.partial = workspace + dot_floats(rows);
   if (dtype == SWIGLU_F32)
     return weight_dtype == SWIGLU_F32 ? launch_bwd<float, float>(p, *d, st) : launch_bwd<float, __nv_bfloat16>(p, *d, st);
   return weight_dtype == SWIGLU_F32 ? launch_bwd<__nv_bfloat16, float>(p, *d, st)
