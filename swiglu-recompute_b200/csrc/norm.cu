@@ -109,6 +109,14 @@ struct RowPacks {
     for (int e = 0; e < V; ++e) f[e] = inside(k, e) ? to_f32(p[at + e]) : 0.0f;
     return set16<T>(f);
   }
+  // Zeros in place of what does not belong to the row.
+  __device__ __forceinline__ uint4 masked(const uint4& u, int k) const {
+    float f[V];
+    get16<T>(u, f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = inside(k, e) ? f[e] : 0.0f;
+    return set16<T>(f);
+  }
   __device__ __forceinline__ void store(T* p, int k, const uint4& u) const {
     const long long at = base - head + static_cast<long long>(k) * V;
     if (!edge(k)) {
@@ -481,45 +489,53 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdLoadRegs<VPT> <= 12 ? 2 : 1)
   }
 }
 
-// The same for rows of whole packs that a block shares (more than a warp): rows
-// arrive through a ring of `stages` rows in shared memory, filled by bulk copies,
-// so that what is in flight does not depend on the registers left (11136 x 3584
-// bf16: registers 60.5 us, ring 56.1; 16384 x 8192: 192, 162; 5000 x 16384: 208,
-// 120; 11136 x 3584 f32: 136, 96).
+// The same for rows that a block shares (more than a warp): rows arrive through a
+// ring of `stages` rows in shared memory, filled by bulk copies, so that what is
+// in flight does not depend on the registers left (11136 x 3584 bf16: registers
+// 60.5 us, ring 56.1; 16384 x 8192: 192, 162; 5000 x 16384: 208, 120; 11136 x 3584
+// f32: 136, 96). SHIFT: a copy takes the row's packs on the 16-byte grid, its
+// neighbours' elements included; they are masked where they are read.
 constexpr int kMaxStages = 8;
 
-template <typename T, typename W, int VPT>
+template <typename T, typename W, int VPT, bool SHIFT>
 __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_ring_kernel(const BwdParams p) {
   wait_for_previous();
   constexpr int V = kV<T>;
-  extern __shared__ __align__(128) uint8_t ring[];  // [stage][dy, s, ds][cols]
+  extern __shared__ __align__(128) uint8_t ring[];  // [stage][dy, s, ds][packs]
   __shared__ uint64_t full[kMaxStages];
   __shared__ float sums[2][32];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
-  const uint32_t row_bytes = static_cast<uint32_t>(p.cols) * sizeof(T);
+  // This block's rows all have the same head: the grid is a multiple of the period.
+  const long long row0 = blockIdx.x, step = gridDim.x;
+  const RowPacks<T, SHIFT> first(row0, p.cols);
+  const int packs = first.packs, warps = static_cast<int>(blockDim.x >> 5);
+  const uint32_t row_bytes = static_cast<uint32_t>(packs) * 16;
   const uint32_t stage_bytes = row_bytes * (p.ds ? 3 : 2);
-  const int packs = p.cols / V, warps = static_cast<int>(blockDim.x >> 5);
-  const long long step = gridDim.x;
+  // The tensor may end inside the last pack of its last row: that pack is not
+  // copied, its owner reads the elements themselves.
+  auto cut = [&](long long row) {
+    return SHIFT && row * p.cols - first.head + static_cast<long long>(packs) * V > p.rows * p.cols;
+  };
   auto fill = [&](int stage, long long row) {  // one thread
     if (row >= p.rows) return;
-    const long long at = row * row_bytes;
+    const long long at = (row * p.cols - first.head) * static_cast<long long>(sizeof(T));
+    const uint32_t bytes = cut(row) ? row_bytes - 16 : row_bytes;
     uint8_t* to = ring + stage * stage_bytes;
-    mbar_arrive_expect_tx(&full[stage], stage_bytes);
-    bulk_load(to, static_cast<const uint8_t*>(p.dy) + at, row_bytes, &full[stage]);
-    bulk_load(to + row_bytes, static_cast<const uint8_t*>(p.s) + at, row_bytes, &full[stage]);
-    if (p.ds) bulk_load(to + 2 * row_bytes, static_cast<const uint8_t*>(p.ds) + at, row_bytes, &full[stage]);
+    mbar_arrive_expect_tx(&full[stage], bytes * (p.ds ? 3 : 2));
+    bulk_load(to, static_cast<const uint8_t*>(p.dy) + at, bytes, &full[stage]);
+    bulk_load(to + row_bytes, static_cast<const uint8_t*>(p.s) + at, bytes, &full[stage]);
+    if (p.ds) bulk_load(to + 2 * row_bytes, static_cast<const uint8_t*>(p.ds) + at, bytes, &full[stage]);
   };
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
     *abort_flag = 0;
     fence_barrier_init();
-    for (int i = 0; i < p.stages; ++i) fill(i, blockIdx.x + i * step);
+    for (int i = 0; i < p.stages; ++i) fill(i, row0 + i * step);
   }
   // Pairs of columns: the arithmetic is on packed f32x2 instructions (the kernel
   // is bound by the instructions it issues, 67 % of the slots without them).
   constexpr int P = V / 2;
-  const RowPacks<T, false> first(0, p.cols);
   float2 w[VPT][P], acc[VPT][P];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -536,8 +552,9 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
   const float inv = 1.0f / static_cast<float>(p.cols);
   int stage = 0, buf = 0;
   uint32_t parity = 0;
-  float next_rstd = blockIdx.x < p.rows ? p.rstd[blockIdx.x] : 0.0f;
-  for (long long row = blockIdx.x; row < p.rows; row += step) {
+  float next_rstd = row0 < p.rows ? p.rstd[row0] : 0.0f;
+  for (long long row = row0; row < p.rows; row += step) {
+    const RowPacks<T, SHIFT> rp(row, p.cols);
     const float rstd = next_rstd;
     const float2 rstd2 = make_float2(rstd, rstd);
     if (row + step < p.rows) next_rstd = p.rstd[row + step];
@@ -553,11 +570,21 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
       const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
       if (k >= packs) continue;
       const int m = kKeep ? i : 0;
-      const uint4 a = at[k], b = at[packs + k];
+      uint4 a = at[k], b = at[packs + k];
+      if (p.ds) ds[i] = at[2 * packs + k];
+      if (SHIFT && first.edge(k)) {
+        if (k + 1 == packs && cut(row)) {
+          a = rp.load(static_cast<const T*>(p.dy), k);
+          b = rp.load(static_cast<const T*>(p.s), k);
+          if (p.ds) ds[i] = rp.load(static_cast<const T*>(p.ds), k);
+        } else {
+          a = first.masked(a, k);
+          b = first.masked(b, k);
+        }
+      }
       if constexpr (!kKeep) dys[i] = a, ss[i] = b;
       pairs16<T>(a, g[m]);
       pairs16<T>(b, v[m]);
-      if (p.ds) ds[i] = at[2 * packs + k];
 #pragma unroll
       for (int e = 0; e < P; ++e) {
         const float2 gv = __fmul2_rn(g[m][e], v[m][e]);
@@ -578,7 +605,6 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
     buf ^= 1;  // a warp may still be reading the other half
     const float c = -(dot * inv * rstd * rstd) * rstd;
     const float2 c2 = make_float2(c, c);
-    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + row * p.cols);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int k = static_cast<int>(threadIdx.x + i * blockDim.x);
@@ -595,7 +621,7 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
         d[e] = __ffma2_rn(v[m][e], c2, d[e]);
         d[e] = __ffma2_rn(__fmul2_rn(g[m][e], rstd2), w[i][e], d[e]);
       }
-      out[k] = unpairs16<T>(d);
+      rp.store(static_cast<T*>(p.dx), k, unpairs16<T>(d));
     }
     if (++stage == p.stages) {
       stage = 0;
@@ -618,8 +644,8 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
     if (k >= packs) continue;
 #pragma unroll
     for (int e = 0; e < P; ++e) {
-      part[k * V + 2 * e] = acc[i][e].x;
-      part[k * V + 2 * e + 1] = acc[i][e].y;
+      if (!SHIFT || first.inside(k, 2 * e)) part[k * V - first.head + 2 * e] = acc[i][e].x;
+      if (!SHIFT || first.inside(k, 2 * e + 1)) part[k * V - first.head + 2 * e + 1] = acc[i][e].y;
     }
   }
 }
@@ -716,10 +742,22 @@ int threads_for(int64_t items, int most) {
   return static_cast<int>(t < 32 ? 32 : t > most ? most : t);
 }
 
+// Packs that a row touches at most, and the rows after which its offset on the
+// 16-byte grid repeats.
+template <typename T, bool SHIFT>
+int64_t most_packs(int64_t cols) {
+  return SHIFT ? (cols + 2 * kV<T> - 2) / kV<T> : cols / kV<T>;
+}
+template <typename T>
+int row_period(int64_t cols) {
+  int period = 1;
+  while (period * cols % kV<T>) period *= 2;
+  return period;
+}
+
 template <typename T, typename W, bool E4M3, int VPT, bool SHIFT>
 bool launch_row(const FwdParams& p, cudaStream_t st) {
-  const int64_t packs = SHIFT ? (p.cols + 2 * kV<T> - 2) / kV<T> : p.cols / kV<T>;
-  const int64_t threads = (packs + VPT - 1) / VPT;
+  const int64_t threads = (most_packs<T, SHIFT>(p.cols) + VPT - 1) / VPT;
   if (threads > kRowThreads) return false;
   const int x = threads_for(threads, kRowThreads);
   const dim3 block(x, x == 32 ? 4 : 1);
@@ -795,8 +833,7 @@ int64_t most_bwd_blocks(int64_t rows, int64_t cols, int sms) {
 
 template <typename T, typename W, int VPT, bool SHIFT>
 bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
-  const int64_t packs = SHIFT ? (p.cols + 2 * kV<T> - 2) / kV<T> : p.cols / kV<T>;
-  const int64_t threads = (packs + VPT - 1) / VPT;
+  const int64_t threads = (most_packs<T, SHIFT>(p.cols) + VPT - 1) / VPT;
   if (threads > kBwdThreads) return false;
   const int x = threads_for(threads, kBwdThreads);
   const dim3 block(x, x == 32 && VPT == 1 ? 8 : 1);
@@ -804,12 +841,9 @@ bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   int64_t grid = static_cast<int64_t>(d.sms) * per_sm;
   const int64_t most = most_bwd_blocks(p.rows, p.cols, d.sms);
   if (grid > most) grid = most;
-  p.period = 1;
-  if (SHIFT) {
-    while (static_cast<int64_t>(p.period) * p.cols % kV<T>) p.period *= 2;
-    grid = grid / p.period * p.period;  // as many blocks for every residue class
-    if (grid == 0) return false;
-  }
+  p.period = SHIFT ? row_period<T>(p.cols) : 1;
+  grid = grid / p.period * p.period;  // as many blocks for every residue class
+  if (grid == 0) return false;
   // No more than one block for every blockDim.y rows of a class.
   const int64_t class_rows = (p.rows + p.period - 1) / p.period;
   const int64_t needed = (class_rows + block.y - 1) / block.y * p.period;
@@ -822,23 +856,25 @@ bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
 
 // Rows of 128 packs or more, at least two of them in the ring: 210 KB of shared
 // memory an SM over the blocks its registers hold.
-template <typename T, typename W, int VPT>
+template <typename T, typename W, int VPT, bool SHIFT>
 bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
-  const int64_t threads = (p.cols / kV<T> + VPT - 1) / VPT;
+  const int64_t packs = most_packs<T, SHIFT>(p.cols), threads = (packs + VPT - 1) / VPT;
   // (60000 x 512 bf16, 64 packs: registers 55.8 us, ring 67.2.)
-  if (p.cols / kV<T> < 128 || threads > kBwdThreads) return false;
+  if (packs < 128 || threads > kBwdThreads) return false;
   const int x = threads_for(threads, kBwdThreads);
   int64_t per_sm = (VPT == 1 ? 1024 : 512) / x;
   const int64_t most = most_bwd_blocks(p.rows, p.cols, d.sms);
   if (per_sm * d.sms > most) per_sm = (most + d.sms - 1) / d.sms;
-  const int64_t stage_bytes = p.cols * sizeof(T) * (p.ds ? 3 : 2);
+  const int64_t stage_bytes = packs * 16 * (p.ds ? 3 : 2);
   int64_t stages = 210 * 1024 / per_sm / stage_bytes;
   if (stages < 2) return false;
   p.stages = static_cast<int>(stages > kMaxStages ? kMaxStages : stages);
-  const int64_t grid = per_sm * d.sms < most ? per_sm * d.sms : most;
-  if (p.rows < 3 * grid) return false;  // a ring pays once a block has several rows to go through
+  int64_t grid = per_sm * d.sms < most ? per_sm * d.sms : most;
+  p.period = SHIFT ? row_period<T>(p.cols) : 1;
+  grid = grid / p.period * p.period;
+  if (grid == 0 || p.rows < 3 * grid) return false;  // a ring pays once a block has several rows to go through
   p.chunks = static_cast<int>(grid);
-  constexpr auto kern = rmsnorm_bwd_ring_kernel<T, W, VPT>;
+  constexpr auto kern = rmsnorm_bwd_ring_kernel<T, W, VPT, SHIFT>;
   KernelState& ks = kernel_state<kern>();
   int dev = 0;
   cudaGetDevice(&dev);
@@ -852,12 +888,9 @@ bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
 
 template <typename T, typename W, bool SHIFT>
 bool launch_bwd_rows(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
-  if constexpr (!SHIFT) {
-    // Two packs a thread first: 11136 x 3584 bf16 56.5 us (one 59.5, four 60.9).
-    if (launch_bwd_ring<T, W, 2>(p, d, st) || launch_bwd_ring<T, W, 1>(p, d, st) || launch_bwd_ring<T, W, 4>(p, d, st))
-      return true;
-  }
-  return launch_bwd_row<T, W, 1, SHIFT>(p, d, st) || launch_bwd_row<T, W, 2, SHIFT>(p, d, st) ||
+  // Two packs a thread first: 11136 x 3584 bf16 56.5 us (one 59.5, four 60.9).
+  return launch_bwd_ring<T, W, 2, SHIFT>(p, d, st) || launch_bwd_ring<T, W, 1, SHIFT>(p, d, st) ||
+         launch_bwd_ring<T, W, 4, SHIFT>(p, d, st) || launch_bwd_row<T, W, 1, SHIFT>(p, d, st) || launch_bwd_row<T, W, 2, SHIFT>(p, d, st) ||
          launch_bwd_row<T, W, 4, SHIFT>(p, d, st);
 }
 

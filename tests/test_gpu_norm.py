@@ -77,7 +77,8 @@ def test_forward_e4m3(M, D, dt, wdt, residual):
     assert torch.all(q.cpu().float().abs().amax(1)[nz] == O.E4M3_MAX)
 
 
-@pytest.mark.parametrize("M,D", SHAPES + [(1500, 520), (2000, 3584)])
+@pytest.mark.parametrize("M,D", SHAPES + [(1500, 520), (2000, 3584), (1201, 1029), (3000, 2051),
+                                            (1000, 8190), (701, 16381), (1777, 1556)])
 @pytest.mark.parametrize("dt,wdt", [(BF, BF), (BF, F32), (F32, F32), (F32, BF)])
 @pytest.mark.parametrize("with_ds", [True, False])
 def test_backward(M, D, dt, wdt, with_ds):

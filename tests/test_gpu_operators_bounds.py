@@ -37,7 +37,7 @@ def _code(dt):
     return _lib.F32 if dt == F32 else _lib.BF16
 
 
-@pytest.mark.parametrize("M,D", [(1, 1), (1, 7), (3, 33), (5, 1001), (2, 4099), (37, 264), (9, 3584), (2, 65544), (700, 520)])
+@pytest.mark.parametrize("M,D", [(1, 1), (1, 7), (3, 33), (5, 1001), (2, 4099), (37, 264), (9, 3584), (2, 65544), (700, 520), (1201, 1029), (1203, 4100)])
 @pytest.mark.parametrize("dt", [BF, F32])
 def test_norm_writes_stay_inside(M, D, dt):
     x, r = torch.randn(M, D, device=DEV).to(dt), torch.randn(M, D, device=DEV).to(dt)
