@@ -854,13 +854,16 @@ bool launch_bwd_row(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   return true;
 }
 
-// Rows of 128 packs or more, at least two of them in the ring: 210 KB of shared
-// memory an SM over the blocks its registers hold.
+// At least two rows in the ring: 210 KB of shared memory an SM over the blocks its
+// registers hold.
 template <typename T, typename W, int VPT, bool SHIFT>
 bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   const int64_t packs = most_packs<T, SHIFT>(p.cols), threads = (packs + VPT - 1) / VPT;
-  // (60000 x 512 bf16, 64 packs: registers 55.8 us, ring 67.2.)
-  if (packs < 128 || threads > kBwdThreads) return false;
+  // Fewer packs: registers. (60000 x 512 bf16, 64 packs: registers 55.8 us, ring
+  // 67.2. Shifted bf16 rows favour the ring earlier: 40000 x 331 registers 98 us, ring
+  // 75; f32 rows do not: 20000 x 501 31.5, 36.8.)
+  const int fewest = SHIFT && sizeof(T) == 2 ? 40 : 128;
+  if (packs < fewest || threads > kBwdThreads) return false;
   const int x = threads_for(threads, kBwdThreads);
   int64_t per_sm = (VPT == 1 ? 1024 : 512) / x;
   const int64_t most = most_bwd_blocks(p.rows, p.cols, d.sms);
