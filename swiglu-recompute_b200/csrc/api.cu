@@ -119,10 +119,8 @@ int current_device(DeviceInfo** out) {
   *out = &d;
   return SWIGLU_OK;
 }
-namespace {
 
 // ------------------------------------------------------------ tensor maps
-}  // namespace
 int get_encode_fn(EncodeTiledFn* out) {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -161,9 +159,9 @@ int make_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, ui
   return SWIGLU_OK;
 }
 
+}  // namespace
 // Output map of a store GEMM: row-major [M, N] (pitch ld elements) in
 // {32 x 32} boxes, 64-byte swizzle for bf16 rows of 64 bytes, 128-byte for f32.
-}  // namespace
 int make_store_map(CUtensorMap* m, void* ptr, uint64_t N, uint64_t M, uint64_t ld, bool f32) {
   EncodeTiledFn fn;
   if (int rc = get_encode_fn(&fn)) return rc;
@@ -328,7 +326,6 @@ bool take_workspace(cudaStream_t st, uint8_t** ptr, size_t* bytes, uint32_t* epo
 // there are idle pairs for (at most kSkMaxSplit, each of at least
 // kSkMinBlocksPerPart blocks), if the stream has a workspace large enough.
 // `slabs` arrival counters are used per tail tile.
-}  // namespace
 void choose_stream_k(int tiles, int clusters, int num_kb, long long tile_floats, int slabs, cudaStream_t st,
                      float** partials, uint32_t** counters, int* tail_out, int* split_out, uint32_t* epoch_out) {
   *tail_out = 0;
@@ -357,7 +354,6 @@ void choose_stream_k(int tiles, int clusters, int num_kb, long long tile_floats,
   *split_out = split;
   *epoch_out = epoch;
 }
-namespace {
 
 template <class Cfg>
 int launch_tc(TcParams& p, const DeviceInfo& d, cudaStream_t st) {

@@ -50,10 +50,6 @@ int check_dtype(int dtype);
 int check_dims(const char* what, int64_t a, int64_t b, int64_t c);
 int check_mult8(const char* what, int64_t v);
 
-// The stream-K tail of a persistent launch, if the stream has a workspace.
-void choose_stream_k(int tiles, int clusters, int num_kb, long long tile_floats, int slabs, cudaStream_t st,
-                     float** partials, uint32_t** counters, int* tail_out, int* split_out, uint32_t* epoch_out);
-
 // Launches a kernel that begins with wait_for_previous(): its blocks may be
 // placed while the stream's previous kernel drains (programmatic dependent
 // launch), which hides the 1-2 us between two kernels of a stream.
