@@ -348,7 +348,10 @@ int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, in
 /* C [M, N] = A . B^T for MXFP4 A [M, K] and B [N, K] with their scales, f32
  * accumulation, C in out_dtype. K % 32 == 0, N % 8 == 0; the MXFP4 form of
  * swiglu_b200_matmul_e4m3. From one row of A up; the sums' order depends on the
- * sizes and the device (and swiglu_b200_set_sm_reserve) alone. */
+ * sizes and the device (and swiglu_b200_set_sm_reserve) alone. Scale bytes beyond
+ * the matrix: those past the last column must be 0, as the quantiser writes them
+ * (they multiply codes of zero; 255 there would make NaN), those past the last
+ * row may hold anything. */
 int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq, const void* b_scale, void* c,
                              int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
 

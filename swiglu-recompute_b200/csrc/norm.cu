@@ -893,8 +893,8 @@ template <typename T, typename W, bool SHIFT>
 bool launch_bwd_rows(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   // Two packs a thread first: 11136 x 3584 bf16 56.5 us (one 59.5, four 60.9).
   return launch_bwd_ring<T, W, 2, SHIFT>(p, d, st) || launch_bwd_ring<T, W, 1, SHIFT>(p, d, st) ||
-         launch_bwd_ring<T, W, 4, SHIFT>(p, d, st) || launch_bwd_row<T, W, 1, SHIFT>(p, d, st) || launch_bwd_row<T, W, 2, SHIFT>(p, d, st) ||
-         launch_bwd_row<T, W, 4, SHIFT>(p, d, st);
+         launch_bwd_ring<T, W, 4, SHIFT>(p, d, st) || launch_bwd_row<T, W, 1, SHIFT>(p, d, st) ||
+         launch_bwd_row<T, W, 2, SHIFT>(p, d, st) || launch_bwd_row<T, W, 4, SHIFT>(p, d, st);
 }
 
 template <typename T, typename W>

@@ -602,7 +602,8 @@ def dequantize_mxfp4(q: torch.Tensor, scale: torch.Tensor, *, dtype: torch.dtype
 def matmul_mxfp4(aq: torch.Tensor, a_scale: torch.Tensor, bq: torch.Tensor, b_scale: torch.Tensor, *,
                  out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """C [M, N] = A . B^T for MXFP4 A [M, K] and B [N, K] with their scales;
-    N % 8 == 0."""
+    N % 8 == 0. Scale bytes past the last column must be 0, as quantize_mxfp4
+    writes them; those past the last row may hold anything."""
     dev = _check_cuda(aq, a_scale, bq, b_scale)
     M, K = _check_mx(aq, a_scale)
     N, K2 = _check_mx(bq, b_scale)
