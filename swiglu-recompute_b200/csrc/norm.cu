@@ -201,14 +201,18 @@ struct FwdParams {
   float eps;
 };
 
-// Row factors from the statistics: rstd, the factor that takes s w to e4m3
-// (clamped, so that a row of tiny values gives 0 * finite and not 0 * inf),
-// and the stored scale: 1 for an all-zero row, NaN where the row holds one.
-__device__ __forceinline__ void row_factors(float sum, float top, const FwdParams& p, float& rstd, float& qs,
-                                            float& scale) {
+// Row factors from the statistics: rstd, the factors that take s w to e4m3, and
+// the stored scale: 1 for an all-zero row, NaN where the row holds one. 448 / top
+// leaves f32 below top = 1.3e-36, so such rows are first multiplied by `lift`
+// (exact), and the scale rounds once, at its end.
+__device__ __forceinline__ void row_factors(float sum, float top, const FwdParams& p, float& rstd, float& lift,
+                                            float& qs, float& scale) {
   rstd = rsqrtf(sum / static_cast<float>(p.cols) + p.eps);
-  qs = top > 0.0f ? fminf(kE4m3Max / top, 3.4028234e38f) : 1.0f;
-  scale = top > 0.0f ? top * rstd / kE4m3Max : (rstd == rstd ? 1.0f : rstd);
+  const bool tiny = top > 0.0f && top < 0x1p-100f;
+  lift = tiny ? 0x1p100f : 1.0f;
+  top *= lift;
+  qs = top > 0.0f ? kE4m3Max / top : 1.0f;
+  scale = top > 0.0f ? top * rstd / kE4m3Max * (tiny ? 0x1p-100f : 1.0f) : (rstd == rstd ? 1.0f : rstd);
 }
 
 // A row in registers: blockDim.x threads hold VPT packs each, all loaded before
@@ -274,11 +278,21 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_fwd_row_kernel(const FwdP
   }
   float sum = sum2.x + sum2.y;
   row_reduce(sum, top, blockDim.x >> 5, scratch);
-  float rstd, qs, scale;
-  row_factors(sum, top, p, rstd, qs, scale);
+  float rstd, lift, qs, scale;
+  row_factors(sum, top, p, rstd, lift, qs, scale);
   if (threadIdx.x == 0) {
     p.rstd[row] = rstd;
     if constexpr (E4M3) p.row_scale[row] = scale;
+  }
+  if constexpr (E4M3) {
+    if (lift != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (static_cast<int>(threadIdx.x + i * blockDim.x) >= rp.packs) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) sw[i][e] *= lift;
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -329,8 +343,8 @@ __global__ void __launch_bounds__(512) rmsnorm_fwd_any_kernel(const FwdParams p)
     if constexpr (E4M3) top = fmaxf(top, fabsf(v * to_f32(w[j])));
   }
   row_reduce(sum, top, blockDim.x >> 5, scratch);
-  float rstd, qs, scale;
-  row_factors(sum, top, p, rstd, qs, scale);
+  float rstd, lift, qs, scale;
+  row_factors(sum, top, p, rstd, lift, qs, scale);
   if (threadIdx.x == 0) {
     p.rstd[blockIdx.x] = rstd;
     if constexpr (E4M3) p.row_scale[blockIdx.x] = scale;
@@ -338,7 +352,7 @@ __global__ void __launch_bounds__(512) rmsnorm_fwd_any_kernel(const FwdParams p)
   const T* src = r ? s : x;
   for (int j = threadIdx.x; j < p.cols; j += blockDim.x) {
     const float v = to_f32(src[j]), f = to_f32(w[j]);
-    if constexpr (E4M3) static_cast<uint8_t*>(p.y)[base + j] = e4m3_byte(v * f * qs);
+    if constexpr (E4M3) static_cast<uint8_t*>(p.y)[base + j] = e4m3_byte(v * f * lift * qs);
     else static_cast<T*>(p.y)[base + j] = from_f32<T>(v * rstd * f);
   }
 }
