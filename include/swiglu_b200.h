@@ -275,8 +275,9 @@ int swiglu_b200_matmul_e4m3(const void* aq, const float* a_scale, const void* bq
  *   rstd [rows] = (mean of s^2 over the row + eps)^-1/2, f32
  *   y = s * rstd * weight, in dtype
  * eps is read on the host during the call (as BLAS scalars are).
- * Statistics are f32. Any cols >= 1; pointers aligned to their element (16-byte
- * alignment of every row takes the faster kernels). s may alias x or residual. */
+ * Statistics are f32. Any cols from 1 to 2^31 - 1025; pointers aligned to their
+ * element (16-byte alignment of every row takes the faster kernels). s may alias x
+ * or residual. */
 int swiglu_b200_rmsnorm_fwd(const void* x, const void* residual, const void* weight, void* y, void* s, float* rstd,
                             int64_t rows, int64_t cols, const float* eps, int dtype, int weight_dtype, void* stream);
 

@@ -741,12 +741,20 @@ __global__ void __launch_bounds__(1024) rmsnorm_dweight_kernel(const float* part
   if (lane == 0 && col < cols) dweight[col] = from_f32<W>(sum);
 }
 
+// The kernels step through a row's columns in ints, up to 1024 at a time.
+constexpr int64_t kMaxCols = 0x7fffffffLL - 1024;
+int check_cols(const char* what, int64_t cols) {
+  if (cols > kMaxCols)
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: at most %lld columns", what, (long long)kMaxCols);
+  return SWIGLU_OK;
+}
+
 int check_norm(const char* what, int64_t rows, int64_t cols, int dtype, int weight_dtype) {
   if (int rc = check_dims(what, rows, cols, 0)) return rc;
   if (int rc = check_dtype(dtype)) return rc;
   if (int rc = check_dtype(weight_dtype)) return rc;
   if (cols == 0) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: a row must have at least one column", what);
-  return SWIGLU_OK;
+  return check_cols(what, cols);
 }
 
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -999,6 +1007,7 @@ int swiglu_b200_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int num_sms, i
   if (int rc = check_dims("rmsnorm_bwd_workspace", rows, cols, num_sms)) return rc;
   if (!floats) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "null pointer");
   if (cols == 0 || num_sms == 0) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "cols and num_sms must be positive");
+  if (int rc = check_cols("rmsnorm_bwd_workspace", cols)) return rc;
   *floats = bwd_floats(rows, cols, num_sms);
   return SWIGLU_OK;
 }
