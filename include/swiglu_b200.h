@@ -338,7 +338,8 @@ int swiglu_b200_clip_grads_by_norm(const void* const* grads, void* const* outs, 
  * [row / 128][block / 4]; bytes beyond the matrix are 0.
  *
  * Quantises src [rows, cols] (F32 or BF16, cols % 32 == 0) into dst
- * [rows, cols / 2] bytes and scale. 16-byte aligned pointers. */
+ * [rows, cols / 2] bytes and scale. 16-byte aligned pointers. Rows and columns of
+ * the MXFP4 calls: at most 2^31 - 256. */
 int swiglu_b200_quantize_mxfp4(const void* src, void* dst, void* scale, int64_t rows, int64_t cols, int dtype,
                                void* stream);
 

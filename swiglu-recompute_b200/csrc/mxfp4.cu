@@ -247,8 +247,13 @@ __global__ void __launch_bounds__(kQuantThreads, 4) dequantize_mxfp4_kernel(cons
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// The kernels round rows and columns up to whole tiles (256 at most) in ints.
+constexpr int64_t kMaxDim = 0x7fffffffLL - 255;
+
 int check_mx(const char* what, int64_t rows, int64_t cols) {
   if (int rc = check_dims(what, rows, cols, 0)) return rc;
+  if (rows > kMaxDim || cols > kMaxDim)
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: at most %lld rows and columns", what, (long long)kMaxDim);
   if (cols % kBlock)
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: %lld columns are not a multiple of 32", what, (long long)cols);
   const int64_t blocks = (rows + kQuantRows - 1) / kQuantRows * ((cols + kQuantCols - 1) / kQuantCols);

@@ -30,3 +30,19 @@ def test_norm_rows_whose_column_numbers_would_overflow(lib, cols):
     _refused(lib, lib.swiglu_b200_rmsnorm_bwd(P, P, P, P, P, P, P, P, 1 << 40, 1, cols, 1, 1, None), b"at most")
     _refused(lib, lib.swiglu_b200_rmsnorm_bwd_workspace(1, cols, 148, ctypes.byref(n)), b"at most")
     assert lib.swiglu_b200_rmsnorm_bwd_workspace(1, TOP - 1024, 148, ctypes.byref(n)) == 0
+
+
+def test_mxfp4_matrices_whose_tiles_would_overflow(lib):
+    """Rows and columns are rounded up to tiles of up to 256 in ints."""
+    wide, tall = 2 ** 31 - 32, 2 ** 31 - 8
+    q, d, m = lib.swiglu_b200_quantize_mxfp4, lib.swiglu_b200_dequantize_mxfp4, lib.swiglu_b200_matmul_mxfp4
+    for f in (q, d):
+        _refused(lib, f(P, P, P, 1, wide, 1, None), b"at most 2147483392 rows and columns")
+        _refused(lib, f(P, P, P, tall, 32, 1, None), b"at most 2147483392 rows and columns")
+    _refused(lib, m(P, P, P, P, P, 1, 8, wide, 1, None), b"at most")
+    _refused(lib, m(P, P, P, P, P, 1, tall, 32, 1, None), b"at most")
+    _refused(lib, m(P, P, P, P, P, tall, 8, 32, 1, None), b"at most")
+    f = lib.swiglu_b200_fused_matmul_swiglu_mxfp4
+    _refused(lib, f(P, P, P, P, P, P, tall, 32, 128, 0, None), b"at most")
+    # an empty matrix of the largest size that is left is no error
+    assert q(None, None, None, 0, 2 ** 31 - 256, 1, None) == 0
