@@ -76,6 +76,10 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, W1, W2, eps, precision):
         ctx.set_materialize_grads(False)
+        # The quantisers take f32 as well, but the backward is that of a bf16 block.
+        if precision != "bf16" and not x.dtype == W1.dtype == W2.dtype == torch.bfloat16:
+            raise TypeError(f"{precision} operands go with a bf16 stream and bf16 parameters, got {x.dtype}, "
+                            f"{W1.dtype}, {W2.dtype}")
         x2 = _flatten_rows(x)
         r2 = None if residual is None else _flatten_rows(residual)
         g, W1c, W2c = weight.contiguous(), W1.contiguous(), W2.contiguous()
@@ -153,8 +157,8 @@ class RMSNormResidual(nn.Module):
 class SwiGLUPreNormBlock(nn.Module):
     """forward(x, residual=None) -> (y, s): s = x + residual (x without one),
     y = MLP(RMSNorm(s)). precision: "bf16" (the parameters' own type: bf16 or
-    f32 kernels), "e4m3" or "mxfp4" (bf16 parameters; MXFP4 wants dim and
-    hidden_dim to be multiples of 32)."""
+    f32 kernels), "e4m3" or "mxfp4" (bf16 parameters and a bf16 stream; MXFP4
+    wants dim and hidden_dim to be multiples of 32)."""
 
     def __init__(self, dim, hidden_dim, out_dim=None, eps=1e-6, dtype=torch.bfloat16, precision="bf16"):
         super().__init__()

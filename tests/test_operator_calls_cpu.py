@@ -3,7 +3,9 @@ no GPU."""
 import ctypes
 
 import pytest
+import torch
 
+import swiglu_block as SB
 from swiglu_b200 import _lib
 
 P = 256
@@ -46,3 +48,20 @@ def test_mxfp4_matrices_whose_tiles_would_overflow(lib):
     _refused(lib, f(P, P, P, P, P, P, tall, 32, 128, 0, None), b"at most")
     # an empty matrix of the largest size that is left is no error
     assert q(None, None, None, 0, 2 ** 31 - 256, 1, None) == 0
+
+
+@pytest.mark.parametrize("precision", ["e4m3", "mxfp4"])
+def test_few_bit_block_wants_a_bf16_stream_and_parameters(precision):
+    """Refused before any kernel runs: an f32 stream or weight used to pass the
+    forward and to fail in the backward, after preact had been overwritten."""
+    b = SB.SwiGLUPreNormBlock(64, 64, precision=precision)
+    x = torch.zeros(4, 64)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            with pytest.raises(TypeError, match="bf16 stream"):
+                b(x, x)
+            with pytest.raises(TypeError, match="bf16 stream"):
+                b(x)
+    b.w2.data = b.w2.data.float()
+    with pytest.raises(TypeError, match="bf16 parameters"):
+        b(x.bfloat16(), x.bfloat16())
