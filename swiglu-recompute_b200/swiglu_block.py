@@ -71,10 +71,12 @@ class RMSNormResidualFunction(torch.autograd.Function):
 
 
 class PreNormSwiGLUFunction(torch.autograd.Function):
-    """(y, s) of the block; without a residual, y alone (s is x)."""
+    """(y, s) of the block; without a residual, y alone (s is x). With grad=False
+    nothing is kept for a backward and preact is not written (a Function's forward
+    cannot see torch.no_grad itself)."""
 
     @staticmethod
-    def forward(ctx, x, residual, weight, W1, W2, eps, precision):
+    def forward(ctx, x, residual, weight, W1, W2, eps, precision, grad=True):
         ctx.set_materialize_grads(False)
         # The quantisers take f32 as well, but the backward is that of a bf16 block.
         if precision != "bf16" and not x.dtype == W1.dtype == W2.dtype == torch.bfloat16:
@@ -83,7 +85,7 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
         x2 = _flatten_rows(x)
         r2 = None if residual is None else _flatten_rows(residual)
         g, W1c, W2c = weight.contiguous(), W1.contiguous(), W2.contiguous()
-        training = any(ctx.needs_input_grad[:5])
+        training = grad and any(ctx.needs_input_grad[:5])
         K = kernels()
         preact = None
         if precision == "e4m3":
@@ -122,7 +124,7 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
         s, g, rstd, W1, W2, preact = ctx.saved_tensors
         need_x, need_r, need_g, need_w1, need_w2 = ctx.needs_input_grad[:5]
         if grad_y is None:  # only the stream was used
-            return ds, ds, None, None, None, None, None
+            return ds, ds, None, None, None, None, None, None
         K = kernels()
         # The norm's output again: the same kernel on the same rows.
         n = K.rmsnorm_fwd(s, g, None, ctx.eps)[0] if need_w1 else None
@@ -137,7 +139,8 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
             d2 = None if ds is None else _flatten_rows(ds).to(s.dtype)
             dx, dg = K.rmsnorm_bwd(dn, s, g, rstd, d2)
             dx = dx.reshape(ctx.x_shape)
-        return (dx if need_x else None, dx if need_r else None, dg if need_g else None, dw1, dw2, None, None)
+        return (dx if need_x else None, dx if need_r else None, dg if need_g else None, dw1, dw2, None, None,
+                None)
 
 
 class RMSNormResidual(nn.Module):
@@ -177,7 +180,8 @@ class SwiGLUPreNormBlock(nn.Module):
 
     def forward(self, x, residual=None):
         _same_stream(x, residual)
-        out = PreNormSwiGLUFunction.apply(x, residual, self.norm_weight, self.w1, self.w2, self.eps, self.precision)
+        out = PreNormSwiGLUFunction.apply(x, residual, self.norm_weight, self.w1, self.w2, self.eps, self.precision,
+                                          torch.is_grad_enabled())
         return (out, x) if residual is None else out
 
 

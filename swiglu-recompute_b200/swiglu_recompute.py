@@ -249,15 +249,17 @@ class SwiGLUFP4ForwardFunction(torch.autograd.Function):
     (bf16) is saved as in SwiGLUMemoryOptimizedFunction, whose bf16 backward
     follows unchanged. No counterpart in the reference; results differ from the
     bf16 block by the e2m1 rounding of the four operands (one mantissa bit).
+    With grad=False nothing is kept for a backward and preact is not written
+    (a Function's forward cannot see torch.no_grad itself).
     """
 
     @staticmethod
-    def forward(ctx, x, W1, W2):
+    def forward(ctx, x, W1, W2, grad=True):
         lead = x.shape[:-1]
         x2 = _flatten_rows(x)
         W1c, W2c = W1.contiguous(), W2.contiguous()
         K = kernels()
-        training = any(ctx.needs_input_grad[:3])
+        training = grad and any(ctx.needs_input_grad[:3])
         preact, h = _mxfp4_gemm1(K, *K.quantize_mxfp4(x2), *K.quantize_mxfp4(W1c), training)
         hq, hs = K.quantize_mxfp4(h)
         del h
@@ -274,7 +276,7 @@ class SwiGLUFP4ForwardFunction(torch.autograd.Function):
         gx, gw1, gw2 = _recompute_backward(ctx, grad_y, x, W1, W2, preact, w_form=W1_ROWS, layout=LAYOUT_STD)
         if gx is not None:
             gx = gx.reshape(ctx.x_shape)
-        return gx, gw1, gw2
+        return gx, gw1, gw2, None
 
 
 # -----------------------------------------------------------------------------
@@ -322,7 +324,7 @@ class SwiGLUMLPFP4Forward(SwiGLUMLPCustom):
     def forward(self, x):
         if x.dtype != torch.bfloat16:
             raise TypeError("the MXFP4 forward takes bf16 activations")
-        return SwiGLUFP4ForwardFunction.apply(x, self.w1, self.w2)
+        return SwiGLUFP4ForwardFunction.apply(x, self.w1, self.w2, torch.is_grad_enabled())
 
 
 class SwiGLUMLPFP4Inference(nn.Module):

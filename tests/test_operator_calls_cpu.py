@@ -5,8 +5,11 @@ import ctypes
 import pytest
 import torch
 
+from torch._subclasses.fake_tensor import FakeTensorMode
+
 import swiglu_block as SB
-from swiglu_b200 import _lib
+import swiglu_recompute as SR
+from swiglu_b200 import _lib, library
 
 P = 256
 TOP = 2 ** 31 - 1
@@ -15,6 +18,23 @@ TOP = 2 ** 31 - 1
 @pytest.fixture(scope="module")
 def lib():
     return _lib.load()
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Names of the kernels that the Functions call; they run as the registered
+    ops' fake forms, on fake tensors."""
+    names = []
+
+    class Recorded:
+        def __getattr__(self, name):
+            names.append(name)
+            return getattr(library._Traced, name)
+
+    for mod in (SR, SB):
+        monkeypatch.setattr(mod, "kernels", lambda: Recorded())
+    with FakeTensorMode():
+        yield names
 
 
 def _refused(lib, rc, text):
@@ -65,3 +85,19 @@ def test_few_bit_block_wants_a_bf16_stream_and_parameters(precision):
     b.w2.data = b.w2.data.float()
     with pytest.raises(TypeError, match="bf16 parameters"):
         b(x.bfloat16(), x.bfloat16())
+
+
+@pytest.mark.parametrize("which", ["fp4", *SB.PRECISIONS])
+def test_evaluation_without_gradients_writes_no_preact(calls, which):
+    """Under torch.no_grad, with parameters that require gradients, the modules take
+    the forms that write h alone; with gradients, those that write preact too."""
+    bf = torch.bfloat16
+    m = SR.SwiGLUMLPFP4Forward(128, 256, dtype=bf) if which == "fp4" else SB.SwiGLUPreNormBlock(128, 256, precision=which)
+    gemm1 = {"fp4": "swiglu_fwd_mxfp4", "mxfp4": "swiglu_fwd_mxfp4", "e4m3": "swiglu_fwd_e4m3", "bf16": "swiglu_fwd"}[which]
+    x = torch.empty(64, 128, dtype=bf)
+    with torch.no_grad():
+        m(x)
+    assert f"{gemm1}_h" in calls and gemm1 not in calls
+    calls.clear()
+    m(x)
+    assert gemm1 in calls and f"{gemm1}_h" not in calls
