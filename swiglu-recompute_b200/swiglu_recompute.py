@@ -256,10 +256,14 @@ class SwiGLUFP4ForwardFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W1, W2, grad=True):
         lead = x.shape[:-1]
+        training = grad and any(ctx.needs_input_grad[:3])
+        # The quantiser takes f32 as well, but the backward is that of a bf16 block.
+        if training and not x.dtype == W1.dtype == W2.dtype == torch.bfloat16:
+            raise TypeError(f"training with MXFP4 operands takes bf16 activations and parameters, got {x.dtype}, "
+                            f"{W1.dtype}, {W2.dtype}")
         x2 = _flatten_rows(x)
         W1c, W2c = W1.contiguous(), W2.contiguous()
         K = kernels()
-        training = grad and any(ctx.needs_input_grad[:3])
         preact, h = _mxfp4_gemm1(K, *K.quantize_mxfp4(x2), *K.quantize_mxfp4(W1c), training)
         hq, hs = K.quantize_mxfp4(h)
         del h
@@ -319,7 +323,8 @@ class SwiGLUMLPFP8Forward(SwiGLUMLPCustom):
 class SwiGLUMLPFP4Forward(SwiGLUMLPCustom):
     """SwiGLUMLPCustom whose forward GEMMs take MXFP4 operands (bf16 weights and
     activations quantised on the fly; dim and hidden_dim multiples of 32); bf16
-    recompute backward."""
+    recompute backward. f32 weights (the constructor's default) serve a forward
+    without gradients alone."""
 
     def forward(self, x):
         if x.dtype != torch.bfloat16:

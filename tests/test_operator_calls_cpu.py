@@ -101,3 +101,16 @@ def test_evaluation_without_gradients_writes_no_preact(calls, which):
     calls.clear()
     m(x)
     assert gemm1 in calls and f"{gemm1}_h" not in calls
+
+
+def test_fp4_training_wants_bf16_parameters():
+    """As the block: f32 weights passed the forward and failed in the backward."""
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    m = SR.SwiGLUMLPFP4Forward(64, 64)
+    half = SR.SwiGLUMLPFP4Forward(64, 64, dtype=torch.bfloat16)
+    half.w2.data = half.w2.data.float()
+    for mlp in (m, half):
+        with pytest.raises(TypeError, match="bf16 activations and parameters"):
+            mlp(x)
+        with pytest.raises(ValueError, match="CUDA"), torch.no_grad():  # allowed as far as the device
+            mlp(x)
