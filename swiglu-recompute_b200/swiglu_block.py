@@ -16,12 +16,11 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from swiglu_b200 import ops
 from swiglu_b200.library import kernels
 from swiglu_b200.ops import LAYOUT_STD, W1_ROWS
-from swiglu_recompute import _flatten_rows, _mxfp4_gemm1, _recompute_backward
+from swiglu_recompute import _first_derivative_only, _flatten_rows, _mxfp4_gemm1, _recompute_backward
 
 PRECISIONS = ("bf16", "e4m3", "mxfp4")
 
@@ -58,7 +57,7 @@ class RMSNormResidualFunction(torch.autograd.Function):
         return y if residual is None else (y, s.reshape(x.shape))
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative_only
     def backward(ctx, dy, ds=None):
         s, w, rstd = ctx.saved_tensors
         if dy is None:
@@ -119,7 +118,7 @@ class PreNormSwiGLUFunction(torch.autograd.Function):
         return y if residual is None else (y, s.reshape(x.shape))
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative_only
     def backward(ctx, grad_y, ds=None):
         s, g, rstd, W1, W2, preact = ctx.saved_tensors
         need_x, need_r, need_g, need_w1, need_w2 = ctx.needs_input_grad[:5]

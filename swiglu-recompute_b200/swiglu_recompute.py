@@ -25,9 +25,12 @@ Shapes:  x [M, D]   W1 [2H, D]   W2 [Dout, H]
 
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from swiglu_b200 import ops
 from swiglu_b200.library import kernels
@@ -61,6 +64,28 @@ def _swiglu_backward_logic(preact: torch.Tensor, grad_h: torch.Tensor) -> torch.
 def _flatten_rows(x: torch.Tensor) -> torch.Tensor:
     x2 = x.reshape(-1, x.shape[-1])
     return x2 if x2.is_contiguous() else x2.contiguous()
+
+
+def _first_derivative_only(backward):
+    """For a Function's backward that cannot be differentiated: gradients taken
+    with create_graph=True raise when they are differentiated again.
+    once_differentiable sees to that only where the incoming gradient requires one;
+    elsewhere the result would be a constant, and a penalty on it would drop out of
+    a loss in silence."""
+    inner = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        out = inner(ctx, *grads)
+        if torch.compiler.is_compiling() or not torch.is_grad_enabled():
+            return out
+        live = [g is not None and not g.requires_grad for g in out]
+        refuse = torch._C._functions.DelayedError(b"this backward has no second derivative", sum(live))
+        marked = iter(refuse(*[g.detach().requires_grad_() for g, mark in zip(out, live) if mark]) if sum(live) > 1 else
+                      [refuse(g.detach().requires_grad_()) for g, mark in zip(out, live) if mark])
+        return tuple(next(marked) if mark else g for g, mark in zip(out, live))
+
+    return wrapper
 
 
 def _recompute_backward(ctx, grad_y, x, w1, w2, preact, *, w_form, layout):
@@ -275,6 +300,7 @@ class SwiGLUFP4ForwardFunction(torch.autograd.Function):
         return y.reshape(*lead, W2.shape[0])
 
     @staticmethod
+    @_first_derivative_only
     def backward(ctx, grad_y):
         x, W1, W2, preact = ctx.saved_tensors
         gx, gw1, gw2 = _recompute_backward(ctx, grad_y, x, W1, W2, preact, w_form=W1_ROWS, layout=LAYOUT_STD)

@@ -114,3 +114,25 @@ def test_fp4_training_wants_bf16_parameters():
             mlp(x)
         with pytest.raises(ValueError, match="CUDA"), torch.no_grad():  # allowed as far as the device
             mlp(x)
+
+
+@pytest.mark.parametrize("which", ["fp4", "norm", *SB.PRECISIONS])
+@pytest.mark.parametrize("leaf", ["x", "all"])
+def test_second_derivatives_are_refused(calls, which, leaf):
+    """A penalty on a gradient used to drop out of a loss in silence."""
+    bf = torch.bfloat16
+    if which == "fp4":
+        m = SR.SwiGLUMLPFP4Forward(64, 64, dtype=bf)
+    else:
+        m = SB.RMSNormResidual(64) if which == "norm" else SB.SwiGLUPreNormBlock(64, 64, precision=which)
+    x = torch.empty(32, 64, dtype=bf, requires_grad=True)
+    params = list(m.parameters())
+    y = m(x) if which in ("fp4", "norm") else m(x)[0]
+    leaves = [x] if leaf == "x" else [x, *params]
+    grads = torch.autograd.grad(y.sum(), leaves, create_graph=True)
+    assert all(g.shape == t.shape and g.dtype == t.dtype for g, t in zip(grads, leaves))
+    for g in grads:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (params[0].square().sum() + g.square().sum()).backward()
+    y = m(x) if which in ("fp4", "norm") else m(x)[0]   # and a plain backward is as before
+    assert not any(g.requires_grad for g in torch.autograd.grad(y.sum(), leaves))
