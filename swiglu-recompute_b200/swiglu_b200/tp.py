@@ -359,6 +359,7 @@ def clip_sharded_grad_norm_(grads, max_norm, device, group=None):
     """ops.clip_grad_norm_ for gradients that are shards: each rank of `group`
     passes its own (none, some or all of them), and all are scaled by the norm
     over all ranks. Returns that norm (f32, on `device`)."""
+    grads = list(grads)
     square = torch.zeros((), dtype=torch.float64, device=device)
     if grads:
         square = ops.grad_norm(grads).double().square()

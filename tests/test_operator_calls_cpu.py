@@ -9,7 +9,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 import swiglu_block as SB
 import swiglu_recompute as SR
-from swiglu_b200 import _lib, library
+from swiglu_b200 import _lib, library, tp
 
 P = 256
 TOP = 2 ** 31 - 1
@@ -136,3 +136,16 @@ def test_second_derivatives_are_refused(calls, which, leaf):
             (params[0].square().sum() + g.square().sum()).backward()
     y = m(x) if which in ("fp4", "norm") else m(x)[0]   # and a plain backward is as before
     assert not any(g.requires_grad for g in torch.autograd.grad(y.sum(), leaves))
+
+
+def test_sharded_clipping_takes_any_iterable(monkeypatch):
+    """A generator was used up by the norm, and the scaling found nothing; an empty
+    one counted as some gradients."""
+    scaled = []
+    monkeypatch.setattr(tp.dist, "all_reduce", lambda t, group=None: None)
+    monkeypatch.setattr(tp.ops, "grad_norm", lambda ts: torch.cat([t.flatten() for t in list(ts)]).norm())
+    monkeypatch.setattr(tp.ops, "clip_grads_by_norm_", lambda ts, norm, max_norm: scaled.extend(ts))
+    grads = [torch.full((4,), 3.0), torch.full((5,), 4.0)]
+    norm = tp.clip_sharded_grad_norm_((g for g in grads), 1.0, torch.device("cpu"))
+    assert abs(norm.item() - (36 + 80) ** 0.5) < 1e-5 and all(a is b for a, b in zip(scaled, grads)) and len(scaled) == 2
+    assert tp.clip_sharded_grad_norm_(iter(()), 1.0, torch.device("cpu")) == 0
