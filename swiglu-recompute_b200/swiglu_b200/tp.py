@@ -355,18 +355,21 @@ def tp_swiglu(x_local, w1_local, w2_local, group=None, compute=NativeCompute, re
     return _TPSwiGLUFunction.apply(x_local, w1_local, w2_local, group, compute, reduce_f32, fused_rs, chunks)
 
 
-def clip_sharded_grad_norm_(grads, max_norm, device, group=None):
+def clip_sharded_grad_norm_(grads, max_norm, device, group=None, replicated=()):
     """ops.clip_grad_norm_ for gradients that are shards: each rank of `group`
     passes its own (none, some or all of them), and all are scaled by the norm
-    over all ranks. Returns that norm (f32, on `device`)."""
-    grads = list(grads)
+    over all ranks. `replicated`: gradients that every rank holds alike (a norm
+    weight's, for instance), which count once and are scaled on every rank; among
+    `grads` they would count once a rank. Returns the norm (f32, on `device`)."""
+    grads, replicated = list(grads), list(replicated)
+    counted = grads + replicated if replicated and dist.get_rank(group) == 0 else grads
     square = torch.zeros((), dtype=torch.float64, device=device)
-    if grads:
-        square = ops.grad_norm(grads).double().square()
+    if counted:
+        square = ops.grad_norm(counted).double().square()
     dist.all_reduce(square, group=group)
     norm = square.sqrt().float()
-    if grads:
-        ops.clip_grads_by_norm_(grads, norm, max_norm)
+    if grads or replicated:
+        ops.clip_grads_by_norm_(grads + replicated, norm, max_norm)
     return norm
 
 

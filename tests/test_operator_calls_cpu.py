@@ -1,9 +1,13 @@
 """Refusals and host-side behaviour of the operators around the block that need
 no GPU."""
 import ctypes
+import os
+import socket
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from torch._subclasses.fake_tensor import FakeTensorMode
 
@@ -149,3 +153,48 @@ def test_sharded_clipping_takes_any_iterable(monkeypatch):
     norm = tp.clip_sharded_grad_norm_((g for g in grads), 1.0, torch.device("cpu"))
     assert abs(norm.item() - (36 + 80) ** 0.5) < 1e-5 and all(a is b for a, b in zip(scaled, grads)) and len(scaled) == 2
     assert tp.clip_sharded_grad_norm_(iter(()), 1.0, torch.device("cpu")) == 0
+
+
+def _replicated_worker(rank, world, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        # the local parts on the CPU; the joining of the ranks is what is tested
+        tp.ops.grad_norm = lambda ts: torch.cat([t.flatten() for t in ts]).double().norm().float()
+
+        def scale(ts, norm, max_norm, out=None):
+            for t in ts:
+                t.mul_(min(1.0, max_norm / (float(norm) + 1e-6)))
+
+        tp.ops.clip_grads_by_norm_ = scale
+        g = torch.Generator().manual_seed(rank)
+        shards = [torch.randn(5, 3, generator=g)] if rank < 2 else []
+        both = [torch.arange(7.0)]
+        keep = [t.clone() for t in shards]
+        norm = tp.clip_sharded_grad_norm_(shards, 0.5, torch.device("cpu"), replicated=both)
+        # by value: a tensor would travel by a handle to memory that the rank takes with it
+        q.put((rank, norm.item(), *([t.tolist() for t in ts] for ts in (keep, shards, both))))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_sharded_clipping_counts_replicated_gradients_once():
+    world = 3
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    procs = [ctx.Process(target=_replicated_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    res = [q.get(timeout=120) for _ in range(world)]
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    every = torch.cat([torch.tensor(t).flatten() for r in res for t in r[2]] + [torch.arange(7.0)]).double()
+    want = every.norm().item()
+    for _, norm, before, after, both in res:
+        assert abs(norm - want) <= 1e-6 * want
+        for a, b in zip([*before, torch.arange(7.0)], [*after, both[0]]):
+            assert torch.allclose(torch.tensor(b), torch.as_tensor(a) * (0.5 / want), rtol=1e-5)
