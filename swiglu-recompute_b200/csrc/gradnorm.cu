@@ -71,7 +71,7 @@ struct ChunkSlots {
   __device__ __forceinline__ long long at(int i) const { return e0 + i * (kGradThreads * N); }
   __device__ __forceinline__ bool inside(int i) const { return at(i) >= 0 && at(i) + N <= size; }
   __device__ __forceinline__ uint4 load_one(int i) const {
-    if (inside(i)) return __ldg(reinterpret_cast<const uint4*>(base + at(i)));
+    if (inside(i)) return *reinterpret_cast<const uint4*>(base + at(i));
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -85,7 +85,7 @@ struct ChunkSlots {
     if (whole) {
       const uint4* p = reinterpret_cast<const uint4*>(base + e0);
 #pragma unroll
-      for (int i = 0; i < kGradSlots; ++i) u[i] = __ldg(p + i * kGradThreads);
+      for (int i = 0; i < kGradSlots; ++i) u[i] = p[i * kGradThreads];
     } else {
 #pragma unroll
       for (int i = 0; i < kGradSlots; ++i) u[i] = load_one(i);

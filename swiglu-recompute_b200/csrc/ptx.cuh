@@ -45,7 +45,9 @@ __device__ __forceinline__ uint32_t warp_id() { return threadIdx.x >> 5; }
 // next kernel's blocks take their places, then waits until the kernels before
 // this one are complete and their writes visible. Nothing may precede it (a
 // waiting block that already held TMEM could keep it from the kernel it waits
-// for).
+// for). Such a kernel is alive while the one before it still writes: it reads
+// through plain loads, not through the read-only path (__ldg, const __restrict__),
+// which asks for data that nobody writes during the kernel's life.
 __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
 }
