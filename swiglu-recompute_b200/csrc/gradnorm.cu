@@ -8,7 +8,8 @@
 // them. The squares of a thread's 64 (bf16) or 32 (f32) values are summed in
 // f32 and everything above that in f64, in an order that depends on sizes
 // only. A thread whose f32 sum leaves the range where f32 squares are safe
-// (values around 1e19 or 1e-15) squares its values again in f64.
+// (values around 1e19 or 1e-15) squares its values again in f64; one whose values
+// are all zeros, told by their bits, is done.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -125,6 +126,10 @@ __device__ __forceinline__ double chunk_squares(const GradTable& t, int k, int c
   }
   const float total = (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
   if (total >= 1e-30f && total <= 1e37f) return static_cast<double>(total);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < kGradSlots; ++i) bits |= u[i].x | u[i].y | u[i].z | u[i].w;
+  if ((bits & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu)) == 0) return 0.0;
   double exact = 0.0;
 #pragma unroll 1
   for (int i = 0; i < kGradSlots; ++i) {  // read again, so that the usual path keeps no values

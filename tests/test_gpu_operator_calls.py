@@ -43,3 +43,25 @@ def test_e4m3_rows_of_tiny_values(D, dt, residual):
              + of_product + of_scale)
     live = top > 0
     assert torch.all(((code * got[:, None] - y).abs() <= bound)[live])
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_zeros_and_values_that_f32_squares_lose_side_by_side(dt):
+    """Zeros of either sign are told from values whose squares underflow f32 by
+    their bits, thread by thread: a lone tiny value among zeros counts, in every
+    slot of a chunk and behind its ragged end. Bounds: one square, two at most, is
+    exact to 2^-53 in f64; the norm rounds once to f32 (2^-24)."""
+    n = 256 * 8 * 8 + 37
+    base = torch.zeros(n, dtype=dt)
+    base[::3] = -0.0
+    assert ops.grad_norm([base.to(DEV)]) == 0
+    for at in (0, 1, 255, 2047, 2048 * 3 + 5, 256 * 8 * 4 - 1, 256 * 8 * 8 - 1, n - 1):
+        for v in (1e-30, -3e-39, 1e-16, 2e19, -1.5):
+            t = base.clone()
+            t[at] = v
+            got = ops.grad_norm([torch.zeros(5, device=DEV), t.to(DEV)])
+            want = t[at].double().abs()
+            assert abs(got.cpu().double() - want) <= max(2 * U * want, 2.0 ** -149), (at, v)
+    for name, z in (("zeros", torch.zeros(100000, dtype=dt)), ("empty end", torch.zeros(3, dtype=dt))):
+        d = [z.to(DEV), torch.ones(4, device=DEV)]
+        assert ops.clip_grad_norm_(d, 1.0) == 2 and not d[0].any(), name
