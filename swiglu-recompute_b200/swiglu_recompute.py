@@ -113,7 +113,8 @@ def _recompute_backward(ctx, grad_y, x, w1, w2, preact, *, w_form, layout):
     if gy.dtype != preact.dtype:
         gy = gy.to(preact.dtype)
     grad_x = grad_w1 = grad_w2 = None
-    emit_h = need_w2 and (need_x or need_w1) and ops.dw2_mode() == "emit_h"
+    rows = preact.shape[0]  # without any, the weights' gradients are empty sums (and no GEMM's K)
+    emit_h = need_w2 and (need_x or need_w1) and ops.dw2_mode() == "emit_h" and rows > 0
     if need_w2 and not emit_h:
         grad_w2 = K.bwd_dw2(gy, preact, layout)
     if need_x or need_w1:
@@ -129,7 +130,9 @@ def _recompute_backward(ctx, grad_y, x, w1, w2, preact, *, w_form, layout):
             del h
         # dW1 and dx contract over the long M and 2H axes: 256 x 512 tiles.
         if need_w1:
-            if w_form == W1_ROWS:
+            if rows == 0:
+                grad_w1 = torch.zeros_like(w1)
+            elif w_form == W1_ROWS:
                 grad_w1 = K.matmul(gp, x, True, False, 512)           # [2H, D] = gp^T x
             else:
                 grad_w1 = K.matmul(x, gp, True, False, 512)           # [D, 2H] = x^T gp

@@ -4,6 +4,8 @@ captured joins, ragged ends."""
 import pytest
 import torch
 
+import swiglu_block as SB
+import swiglu_recompute as SR
 from oracle import operators as O
 from swiglu_b200 import ops
 
@@ -65,3 +67,31 @@ def test_zeros_and_values_that_f32_squares_lose_side_by_side(dt):
     for name, z in (("zeros", torch.zeros(100000, dtype=dt)), ("empty end", torch.zeros(3, dtype=dt))):
         d = [z.to(DEV), torch.ones(4, device=DEV)]
         assert ops.clip_grad_norm_(d, 1.0) == 2 and not d[0].any(), name
+
+
+@pytest.mark.parametrize("which", ["mlp", "fp8", "fp4", "norm", *SB.PRECISIONS])
+@pytest.mark.parametrize("mode", ops.DW2_MODES)
+def test_training_without_rows(which, mode):
+    """An expert without tokens, an empty last batch: empty outputs, gradients of
+    zeros (the weights' gradient used to be refused for its empty sum)."""
+    made = {"mlp": SR.SwiGLUMLPCustom, "fp8": SR.SwiGLUMLPFP8Forward, "fp4": SR.SwiGLUMLPFP4Forward}
+    if which in made:
+        m = made[which](64, 128, 96, dtype=BF)
+    else:
+        m = SB.RMSNormResidual(64) if which == "norm" else SB.SwiGLUPreNormBlock(64, 128, 96, precision=which)
+    m.to(DEV)
+    x = torch.empty(0, 5, 64, device=DEV, dtype=BF, requires_grad=True)
+    ops.set_dw2_mode(mode)
+    try:
+        if which in made:
+            outs = [m(x)]
+        else:
+            r = torch.empty_like(x, requires_grad=True)
+            outs = list(m(x, r))
+        assert outs[0].shape == (0, 5, 64 if which == "norm" else 96)
+        torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
+    finally:
+        ops.set_dw2_mode("prologue")
+    assert x.grad.shape == x.shape
+    for p in m.parameters():
+        assert p.grad.shape == p.shape and p.grad.dtype == p.dtype and not p.grad.any()
