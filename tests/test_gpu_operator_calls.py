@@ -1,13 +1,15 @@
 """Calls of the operators around the block that their documentation allows and
 that are easily got wrong: the ends of the range, rows and gradients of zeros,
 captured joins, ragged ends."""
+import ctypes
+
 import pytest
 import torch
 
 import swiglu_block as SB
 import swiglu_recompute as SR
 from oracle import operators as O
-from swiglu_b200 import ops
+from swiglu_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +97,114 @@ def test_training_without_rows(which, mode):
     assert x.grad.shape == x.shape
     for p in m.parameters():
         assert p.grad.shape == p.shape and p.grad.dtype == p.dtype and not p.grad.any()
+
+
+# Rows of odd widths through the shared-memory ring (at least three rows a block),
+# with every number of elements that a matrix can leave in its last pack.
+RAGGED = ([(3000 + k, 2051, F32) for k in (1, 2, 3)] + [(445, 4095, F32), (446, 4095, F32)]
+          + [(3000 + k, 1029, BF) for k in range(1, 8)] + [(445, 8191, BF), (450, 8190, BF)])
+
+
+@pytest.mark.parametrize("M,D,dt", RAGGED)
+@pytest.mark.parametrize("with_ds", [True, False])
+def test_norm_gradient_of_a_matrix_that_ends_inside_a_pack(M, D, dt, with_ds):
+    """dx and dweight to the bounds of the norm's own tests, and nothing written
+    behind or before dx."""
+    assert M * D % (128 // torch.finfo(dt).bits) != 0
+    g = torch.Generator().manual_seed(M + D)
+    s, dy = torch.randn(M, D, generator=g).to(dt), torch.randn(M, D, generator=g).to(dt)
+    ds = (torch.randn(M, D, generator=g) * 0.25).to(dt) if with_ds else None
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(dt)
+    rstd = O.rmsnorm(s, w)[2].float()
+    es, guard = s.element_size(), 256
+    raw = torch.full((M * D * es + 2 * guard,), 0xA5, dtype=torch.uint8, device=DEV)
+    dx = raw[guard:guard + M * D * es].view(dt).view(M, D)
+    dw = torch.empty(D, device=DEV, dtype=dt)
+    n = ctypes.c_int64(0)
+    _lib.call("swiglu_b200_rmsnorm_bwd_workspace", M, D, ops._num_sms(0), ctypes.byref(n))
+    ws = torch.empty(n.value, device=DEV)
+    code = _lib.F32 if dt == F32 else _lib.BF16
+    a = [None if t is None else t.to(DEV) for t in (dy, s, w, rstd, ds)]
+    _lib.call("swiglu_b200_rmsnorm_bwd", *(None if t is None else t.data_ptr() for t in a), dx.data_ptr(), dw.data_ptr(),
+              ws.data_ptr(), n.value, M, D, code, code, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert bool((raw[:guard] == 0xA5).all()) and bool((raw[guard + M * D * es:] == 0xA5).all())
+    rx, rw = O.rmsnorm_grad(dy, s, w, rstd, ds)
+    half, r = torch.finfo(dt).eps / 2, rstd.double()[:, None]
+    gw, S = (dy.double() * w.double()).abs(), s.double().abs()
+    along = S * r ** 3 * (gw * S).mean(1, keepdim=True)
+    size = r * gw + along + (0 if ds is None else ds.double().abs())
+    assert torch.all((dx.cpu().double() - rx).abs() <= half * rx.abs() + (D / 32 + 48) * U * along + 8 * U * size)
+    mass = (dy.double().abs() * S * r).sum(0)
+    assert torch.all((dw.cpu().double() - rw).abs() <= half * rw.abs() + (M + 48) * U * mass)
+    assert ops.device_status(0) == 0
+
+
+def test_captured_behind_a_join_of_two_streams():
+    """Kernels that are placed early (programmatic dependent launch) behind a fork and
+    a join in a captured graph: the eager call's bits, replayed on other inputs."""
+    g = torch.Generator().manual_seed(4)
+    new = lambda: [torch.randn(700, 512, generator=g).to(BF).to(DEV) for _ in range(2)]  # noqa: E731
+    x, r = new()
+    w = torch.ones(512, device=DEV, dtype=BF)
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        q, scale = ops.quantize_mxfp4(x)
+        with torch.cuda.stream(side):
+            y, s, rstd = ops.rmsnorm_fwd(r, w, x)
+        main.wait_stream(side)
+        dx, dw = ops.rmsnorm_bwd(y, s, w, rstd, x)       # directly behind the join
+        back = ops.dequantize_mxfp4(q, scale)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            c = ops.matmul_mxfp4(q, scale, q[:64], scale[:1])
+        norm = ops.clip_grad_norm_([dx, dw, back], 1.0)
+        main.wait_stream(side)
+        return y, s, dx, dw, back, c, norm
+
+    for _ in range(2):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        for a, b in zip((x, r), new()):
+            a.copy_(b)
+        want = [t.clone() for t in step()]
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert ops.device_status(0) == 0
+
+
+@pytest.mark.parametrize("which", ["fp4", "served", "norm", *SB.PRECISIONS])
+def test_modules_compile_with_and_without_gradients(which):
+    """torch.compile gives the eager bits, in training and under torch.no_grad."""
+    torch.manual_seed(3)
+    x, r = (torch.randn(96, 128, device=DEV).to(BF) for _ in range(2))
+    if which in ("fp4", "served"):
+        m = SR.SwiGLUMLPFP4Forward(128, 256, dtype=BF).to(DEV)
+        m = SR.SwiGLUMLPFP4Inference.from_mlp(m) if which == "served" else m
+        args = (x,)
+    else:
+        m = SB.RMSNormResidual(128).to(DEV) if which == "norm" else SB.SwiGLUPreNormBlock(128, 256, precision=which).to(DEV)
+        args = (x, r)
+    torch._dynamo.reset()
+    c = torch.compile(m, fullgraph=True)
+    outs = lambda f: [f(*args)] if len(args) == 1 else list(f(*args))  # noqa: E731
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(outs(c), outs(m)))
+    params = list(m.parameters())
+    if params:
+        a, b = outs(m), outs(c)
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+        ga, gb = (torch.autograd.grad(o[0].float().square().sum(), params) for o in (a, b))
+        assert all(torch.equal(u, v) for u, v in zip(ga, gb))
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(outs(c), outs(m)))
