@@ -377,7 +377,9 @@ struct BwdParams {
 };
 
 // Threads of a backward row, and the registers its three loads take: up to 12,
-// two blocks of 512 threads fit an SM; up to 24, the next row's loads fit too.
+// two blocks of 512 threads fit an SM; up to 24, the next row's loads fit too. (The
+// compiler reports spills for bf16 rows: one shifted pack 20 bytes a thread, two
+// packs 16, four packs 64 to 324; none for f32.)
 constexpr int kBwdThreads = 512;
 template <int VPT>
 constexpr int kBwdLoadRegs = 12 * VPT;
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kBwdThreads, kBwdLoadRegs<VPT> <= 12 ? 2 : 1)
 constexpr int kMaxStages = 8;
 
 template <typename T, typename W, int VPT, bool SHIFT>
-__global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_ring_kernel(const BwdParams p) {
+__global__ void __launch_bounds__(kBwdThreads, 1) rmsnorm_bwd_ring_kernel(const BwdParams p) {
   wait_for_previous();
   constexpr int V = kV<T>;
   extern __shared__ __align__(128) uint8_t ring[];  // [stage][dy, s, ds][packs]
@@ -574,7 +576,9 @@ __global__ void __launch_bounds__(kBwdThreads, VPT == 1 ? 2 : 1) rmsnorm_bwd_rin
     if (row + step < p.rows) next_rstd = p.rstd[row + step];
     const bool ok = mbar_wait(&full[stage], parity, abort_flag, p.status, kErrTimeoutProducer);
     const uint4* at = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
-    // Four packs stay as loaded and are taken apart twice: as f32 they would spill.
+    // Four packs stay as loaded and are taken apart twice: as f32, bf16 would need 32
+    // registers more. The compiler reports 24 bytes of spills a thread for bf16 even
+    // so (shifted 72), none for f32.
     constexpr bool kKeep = VPT <= 2;
     float2 g[kKeep ? VPT : 1][P], v[kKeep ? VPT : 1][P];
     uint4 dys[kKeep ? 1 : VPT], ss[kKeep ? 1 : VPT], ds[VPT];
@@ -887,7 +891,7 @@ bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   const int fewest = SHIFT && sizeof(T) == 2 ? 40 : 128;
   if (packs < fewest || threads > kBwdThreads) return false;
   const int x = threads_for(threads, kBwdThreads);
-  int64_t per_sm = (VPT == 1 ? 1024 : 512) / x;
+  int64_t per_sm = kBwdThreads / x;
   const int64_t most = most_bwd_blocks(p.rows, p.cols, d.sms);
   if (per_sm * d.sms > most) per_sm = (most + d.sms - 1) / d.sms;
   const int64_t stage_bytes = packs * 16 * (p.ds ? 3 : 2);
@@ -913,10 +917,11 @@ bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
 
 template <typename T, typename W, bool SHIFT>
 bool launch_bwd_rows(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
-  // Two packs a thread first: 11136 x 3584 bf16 56.5 us (one 59.5, four 60.9).
-  return launch_bwd_ring<T, W, 2, SHIFT>(p, d, st) || launch_bwd_ring<T, W, 1, SHIFT>(p, d, st) ||
-         launch_bwd_ring<T, W, 4, SHIFT>(p, d, st) || launch_bwd_row<T, W, 1, SHIFT>(p, d, st) ||
-         launch_bwd_row<T, W, 2, SHIFT>(p, d, st) || launch_bwd_row<T, W, 4, SHIFT>(p, d, st);
+  // Two packs a thread first: 11136 x 3584 bf16 56.5 us (four 60.9; one took 59.5, and
+  // no shape that two packs refuse).
+  return launch_bwd_ring<T, W, 2, SHIFT>(p, d, st) || launch_bwd_ring<T, W, 4, SHIFT>(p, d, st) ||
+         launch_bwd_row<T, W, 1, SHIFT>(p, d, st) || launch_bwd_row<T, W, 2, SHIFT>(p, d, st) ||
+         launch_bwd_row<T, W, 4, SHIFT>(p, d, st);
 }
 
 template <typename T, typename W>
