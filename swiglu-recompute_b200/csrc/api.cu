@@ -25,22 +25,6 @@ namespace {
 
 thread_local std::string t_last_error;
 
-}  // namespace
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  t_last_error = buf;
-  return code;
-}
-
-int cuda_fail(cudaError_t e, const char* what) {
-  return fail(SWIGLU_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
-}
-namespace {
-
 // Tile-order group (in 128-row tiles) for the GEMMs whose caller passes none:
 // 32 (16 pair rows) measured at config 2 against 16: GEMM1 1.618 -> 1.590 ms
 // with DRAM reads 1.87 -> 1.06 GB, y/dW1/dx within 0.2 %; walking every row
@@ -92,7 +76,28 @@ int resolve_device(int* out) {
   return SWIGLU_OK;
 }
 
+// SMs the persistent launches leave free (swiglu_b200_set_sm_reserve), so
+// that kernels of other streams, e.g. NCCL collectives overlapped with the
+// GEMMs, find SMs to run on.
+std::atomic<int> g_sm_reserve{0};
+
 }  // namespace
+
+// ------------------------------------------- shared with the other units (host.cuh)
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  t_last_error = buf;
+  return code;
+}
+
+int cuda_fail(cudaError_t e, const char* what) {
+  return fail(SWIGLU_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
+}
+
 int current_device(DeviceInfo** out) {
   int dev = 0;
   cudaError_t e = cudaSuccess;
@@ -120,7 +125,24 @@ int current_device(DeviceInfo** out) {
   return SWIGLU_OK;
 }
 
-// ------------------------------------------------------------ tensor maps
+int sm_reserve() { return g_sm_reserve.load(std::memory_order_relaxed); }
+
+int check_dtype(int dtype) {
+  if (dtype != SWIGLU_F32 && dtype != SWIGLU_BF16) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  return SWIGLU_OK;
+}
+
+int check_dims(const char* what, int64_t a, int64_t b, int64_t c) {
+  if (!fits_int(a) || !fits_int(b) || !fits_int(c))
+    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: dimensions must be in [0, 2^31)", what);
+  return SWIGLU_OK;
+}
+
+int check_mult8(const char* what, int64_t v) {
+  if (v % 8) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s=%lld must be a multiple of 8", what, (long long)v);
+  return SWIGLU_OK;
+}
+
 int get_encode_fn(EncodeTiledFn* out) {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -135,8 +157,50 @@ int get_encode_fn(EncodeTiledFn* out) {
   *out = fn;
   return SWIGLU_OK;
 }
+
+// Output map of a store GEMM: row-major [M, N] (pitch ld elements) in
+// {32 x 32} boxes, 64-byte swizzle for bf16 rows of 64 bytes, 128-byte for f32.
+int make_store_map(CUtensorMap* m, void* ptr, uint64_t N, uint64_t M, uint64_t ld, bool f32) {
+  EncodeTiledFn fn;
+  if (int rc = get_encode_fn(&fn)) return rc;
+  const uint64_t es = f32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(ptr) % 16) return fail(SWIGLU_ERR_MISALIGNED, "C: base address is not 16-byte aligned");
+  if ((ld * es) % 16) return fail(SWIGLU_ERR_MISALIGNED, "C: row pitch is not a multiple of 16 bytes");
+  const cuuint64_t dims[2] = {N, M};
+  const cuuint64_t strides[1] = {ld * es};
+  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides,
+                  box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "C: cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+  return SWIGLU_OK;
+}
+
+int make_map_bytes(CUtensorMap* m, const void* ptr, uint64_t K, uint64_t rows, uint64_t ld, uint32_t box_rows,
+                  const char* what) {
+  EncodeTiledFn fn;
+  if (int rc = get_encode_fn(&fn)) return rc;
+  if (reinterpret_cast<uintptr_t>(ptr) % 16)
+    return fail(SWIGLU_ERR_MISALIGNED, "%s: base address is not 16-byte aligned", what);
+  if (ld % 16)
+    return fail(SWIGLU_ERR_MISALIGNED, "%s: row pitch of %llu bytes is not a multiple of 16", what,
+                (unsigned long long)ld);
+  const cuuint64_t dims[2] = {K, rows};
+  const cuuint64_t strides[1] = {ld};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t es[2] = {1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
+  return SWIGLU_OK;
+}
+
 namespace {
 
+// ------------------------------------------------------------ tensor maps
 // 2-D bf16 map over a row-major [outer, inner] view with row pitch `ld`
 // elements; 128-byte swizzled boxes of {64, box_outer}.
 int make_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_outer,
@@ -158,28 +222,6 @@ int make_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, ui
   if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
   return SWIGLU_OK;
 }
-
-}  // namespace
-// Output map of a store GEMM: row-major [M, N] (pitch ld elements) in
-// {32 x 32} boxes, 64-byte swizzle for bf16 rows of 64 bytes, 128-byte for f32.
-int make_store_map(CUtensorMap* m, void* ptr, uint64_t N, uint64_t M, uint64_t ld, bool f32) {
-  EncodeTiledFn fn;
-  if (int rc = get_encode_fn(&fn)) return rc;
-  const uint64_t es = f32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(ptr) % 16) return fail(SWIGLU_ERR_MISALIGNED, "C: base address is not 16-byte aligned");
-  if ((ld * es) % 16) return fail(SWIGLU_ERR_MISALIGNED, "C: row pitch is not a multiple of 16 bytes");
-  const cuuint64_t dims[2] = {N, M};
-  const cuuint64_t strides[1] = {ld * es};
-  const cuuint32_t box[2] = {32, 32};
-  const cuuint32_t elem[2] = {1, 1};
-  CUresult r = fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides,
-                  box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "C: cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
-  return SWIGLU_OK;
-}
-namespace {
 
 // 4-D bf16 map gathering several 64-column blocks of a row-major matrix in
 // one TMA operation: dims {64 columns, rows, blocks, groups} with byte
@@ -205,28 +247,6 @@ int make_map_gather4(CUtensorMap* m, const void* ptr, uint64_t rows, uint64_t ld
   return SWIGLU_OK;
 }
 
-}  // namespace
-int make_map_bytes(CUtensorMap* m, const void* ptr, uint64_t K, uint64_t rows, uint64_t ld, uint32_t box_rows,
-                  const char* what) {
-  EncodeTiledFn fn;
-  if (int rc = get_encode_fn(&fn)) return rc;
-  if (reinterpret_cast<uintptr_t>(ptr) % 16)
-    return fail(SWIGLU_ERR_MISALIGNED, "%s: base address is not 16-byte aligned", what);
-  if (ld % 16)
-    return fail(SWIGLU_ERR_MISALIGNED, "%s: row pitch of %llu bytes is not a multiple of 16", what,
-                (unsigned long long)ld);
-  const cuuint64_t dims[2] = {K, rows};
-  const cuuint64_t strides[1] = {ld};
-  const cuuint32_t box[2] = {128, box_rows};
-  const cuuint32_t es[2] = {1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, es,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(SWIGLU_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
-  return SWIGLU_OK;
-}
-namespace {
-
 // Operand maps. K-major operand stored [rows][K]; MN-major stored [K][cols].
 int map_kmajor(CUtensorMap* m, const void* p, int64_t rows, int64_t K, int64_t ld, uint32_t box_rows,
                const char* what) {
@@ -243,14 +263,6 @@ constexpr uint32_t kMnSbo = 8 * 128;      // eight 128-byte swizzle rows
 // GEMM kernel choice: 0 = by size, 1 = single-SM kernel, 2 = 2-SM kernel with
 // 256 x 256 tiles, 3 = 2-SM kernel with 256 x 512 tiles.
 std::atomic<int> g_gemm_path{0};
-
-// SMs the persistent launches leave free (swiglu_b200_set_sm_reserve), so
-// that kernels of other streams, e.g. NCCL collectives overlapped with the
-// GEMMs, find SMs to run on.
-std::atomic<int> g_sm_reserve{0};
-}  // namespace
-int sm_reserve() { return g_sm_reserve.load(std::memory_order_relaxed); }
-namespace {
 
 // ------------------------------------------------------------ stream-K workspaces
 // A caller-owned device buffer per (device, stream), registered with
@@ -475,14 +487,6 @@ int pointwise_grid(long long work, const DeviceInfo& d) {
   return g < 1 ? 1 : static_cast<int>(g);
 }
 
-
-
-}  // namespace
-int check_dtype(int dtype) {
-  if (dtype != SWIGLU_F32 && dtype != SWIGLU_BF16) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
-  return SWIGLU_OK;
-}
-namespace {
 int check_layout(int layout, int64_t H) {
   if (layout != SWIGLU_LAYOUT_STD && layout != SWIGLU_LAYOUT_PACKED128)
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "unknown layout %d", layout);
@@ -490,17 +494,6 @@ int check_layout(int layout, int64_t H) {
     return fail(SWIGLU_ERR_INVALID_ARGUMENT, "packed layout needs H %% 128 == 0 (H=%lld)", (long long)H);
   return SWIGLU_OK;
 }
-}  // namespace
-int check_dims(const char* what, int64_t a, int64_t b, int64_t c) {
-  if (!fits_int(a) || !fits_int(b) || !fits_int(c))
-    return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s: dimensions must be in [0, 2^31)", what);
-  return SWIGLU_OK;
-}
-int check_mult8(const char* what, int64_t v) {
-  if (v % 8) return fail(SWIGLU_ERR_INVALID_ARGUMENT, "%s=%lld must be a multiple of 8", what, (long long)v);
-  return SWIGLU_OK;
-}
-namespace {
 
 // ---------------------------------------------------------------- ops
 int op_swiglu_fwd(const void* x, const void* w, void* preact, void* h, int64_t M, int64_t K, int64_t H, int dtype,

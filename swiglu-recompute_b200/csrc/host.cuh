@@ -26,7 +26,6 @@ struct DeviceInfo {
   uint32_t* status = nullptr;
 };
 
-
 // The device of the calling thread's context, checked to be a B200.
 int current_device(DeviceInfo** out);
 
@@ -36,7 +35,6 @@ int sm_reserve();
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 
 int get_encode_fn(EncodeTiledFn* out);
 // 8-bit operand map: row-major [rows, K] bytes, row pitch `ld` bytes; 128-byte
@@ -81,18 +79,25 @@ KernelState& kernel_state() {
   return s;
 }
 
-// Persistent single-CTA launch: one CTA per SM (at most one per tile).
-template <auto kern, class Params>
-int launch_single(const Params& p, int tiles, int threads, int smem, const DeviceInfo& d, cudaStream_t st,
-                  const char* what) {
+// Lets a kernel have `bytes` of dynamic shared memory, once per device.
+template <auto kern>
+int opt_in_smem(int bytes, const char* what) {
   KernelState& ks = kernel_state<kern>();
   int dev = 0;
   cudaGetDevice(&dev);
   if (!(ks.ready.load() & (1ull << dev))) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return cuda_fail(e, what);
     ks.ready.fetch_or(1ull << dev);
   }
+  return SWIGLU_OK;
+}
+
+// Persistent single-CTA launch: one CTA per SM (at most one per tile).
+template <auto kern, class Params>
+int launch_single(const Params& p, int tiles, int threads, int smem, const DeviceInfo& d, cudaStream_t st,
+                  const char* what) {
+  if (int rc = opt_in_smem<kern>(smem, what)) return rc;
   int sms = d.sms - sm_reserve();
   if (sms < 1) sms = 1;
   const int grid = tiles < sms ? tiles : sms;

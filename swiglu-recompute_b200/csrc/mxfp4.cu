@@ -398,14 +398,7 @@ template <int NT, bool F32>
 int launch_cluster(const MxClusterParams& p, const MxPlan& plan, cudaStream_t st) {
   using Cfg = MxClusterCfg<NT, F32>;
   constexpr auto kern = mx_gemm_cluster_kernel<Cfg>;
-  KernelState& ks = kernel_state<kern>();
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!(ks.ready.load() & (1ull << dev))) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
-    if (e != cudaSuccess) return cuda_fail(e, "matmul_mxfp4 launch");
-    ks.ready.fetch_or(1ull << dev);
-  }
+  if (int rc = opt_in_smem<kern>(Cfg::SMEM_BYTES, "matmul_mxfp4 launch")) return rc;
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = pair_launch_config(attr, Cfg::NUM_THREADS, Cfg::SMEM_BYTES, st);
   attr[0].val.clusterDim.x = plan.parts;

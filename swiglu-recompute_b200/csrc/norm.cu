@@ -904,13 +904,7 @@ bool launch_bwd_ring(BwdParams& p, const DeviceInfo& d, cudaStream_t st) {
   if (grid == 0 || p.rows < 3 * grid) return false;  // a ring pays once a block has several rows to go through
   p.chunks = static_cast<int>(grid);
   constexpr auto kern = rmsnorm_bwd_ring_kernel<T, W, VPT, SHIFT>;
-  KernelState& ks = kernel_state<kern>();
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (!(ks.ready.load() & (1ull << dev))) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 212 * 1024) != cudaSuccess) return false;
-    ks.ready.fetch_or(1ull << dev);
-  }
+  if (opt_in_smem<kern>(212 * 1024, "rmsnorm backward launch")) return false;
   launch_after(kern, p.chunks, x, p.stages * stage_bytes, st, p);
   return true;
 }
