@@ -363,7 +363,8 @@ int swiglu_b200_matmul_mxfp4(const void* aq, const void* a_scale, const void* bq
  * H % 128 == 0. One launch where the product takes pair tiles (the plan query,
  * host-only, sets *fused to 1): preact or h may then be NULL. Elsewhere (few
  * rows) the product is followed by swiglu_b200_forward_logic and preact must be
- * given. */
+ * given. The two forms' sigmoids differ within a few f32 ulp, so the last bit of
+ * h may differ between them. */
 int swiglu_b200_fused_matmul_swiglu_mxfp4_plan(int64_t M, int64_t K, int64_t H, int num_sms, int* fused);
 int swiglu_b200_fused_matmul_swiglu_mxfp4(const void* xq, const void* x_scale, const void* w1q, const void* w1_scale,
                                           void* preact, void* h, int64_t M, int64_t K, int64_t H, int layout,

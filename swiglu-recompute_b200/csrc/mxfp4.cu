@@ -342,10 +342,10 @@ struct MxPlan {
 
 // Times in us, fitted to measurements of every form on one B200 (148 SMs) over
 // 40 shapes (M 1..4096, N 128..28672, K 512..28672), most within 15 %:
-//   pair     5.2 + rounds * (0.37 a k-block + 1)
+//   pair     4.2 + rounds * (0.37 a k-block + 1)
 //   cluster  per wave of two CTAs an SM, start and end, 0.35..0.43 a k-block of
 //            a CTA (half as much again while two share an SM), and the join
-// e.g. 256 x 3584 x 3584: pair 10.6, 128 columns on one CTA 12.6, on two 10.6;
+// Measured, e.g. 256 x 3584 x 3584: pair 10.6, 128 columns on one CTA 12.6, on two 10.6;
 // 333 x 1000 x 14336: pair 24.3, 128 on one 29.2, on four 12.6, on eight 12.4;
 // 1024 x 3584 x 3584: pair 11.0, 128 on one 15.3; 1 x 3584 x 14336: 16 columns
 // on one CTA 23.0, on two 14.3, on four 10.1, on eight 9.5.

@@ -126,7 +126,9 @@ __device__ __forceinline__ void mx_swiglu_chunk(const MxParams& p, const uint32_
   if (p.store_h) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      // From the rounded preact, as the pointwise kernel of the other form.
+      // From the rounded preact, as the pointwise kernel of the other form; that one
+      // has expf and a division in place of sigmoid_fast (as everywhere in this
+      // library), so the last bit of a row's h may depend on the number of rows.
       const float l = bf16_round(__uint_as_float(rl[i])), g = bf16_round(__uint_as_float(rg[i]));
       v[i] = l * (g * sigmoid_fast(g));
     }

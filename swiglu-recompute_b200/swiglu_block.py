@@ -188,9 +188,11 @@ class SwiGLUPreNormBlock(nn.Module):
 def clip_grad_norm_(parameters, max_norm):
     """Scales the gradients of `parameters` (an iterable of tensors, or one) in
     place by min(1, max_norm / (norm + 1e-6)) and returns their global 2-norm,
-    on the device. The signature of torch.nn.utils.clip_grad_norm_ for its
-    2-norm; parameters without a gradient are skipped, and without any the norm
-    is zero."""
+    on the device. It stands in for torch.nn.utils.clip_grad_norm_(parameters,
+    max_norm); norm_type (always 2), error_if_nonfinite and foreach are not taken.
+    Gradients are dense, bf16 or f32, on one device; a parameter may be listed once
+    only. Parameters without a gradient are skipped, and without any the norm is
+    zero."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
