@@ -343,7 +343,8 @@ int swiglu_b200_clip_grads_by_norm(const void* const* grads, void* const* outs, 
 int swiglu_b200_quantize_mxfp4(const void* src, void* dst, void* scale, int64_t rows, int64_t cols, int dtype,
                                void* stream);
 
-/* The values that codes and scales stand for, in dtype (exact). */
+/* The values that codes and scales stand for, in dtype: exact (scale bytes 253
+ * and 254, which the quantiser never writes, may leave the type's range). */
 int swiglu_b200_dequantize_mxfp4(const void* q, const void* scale, void* dst, int64_t rows, int64_t cols, int dtype,
                                  void* stream);
 

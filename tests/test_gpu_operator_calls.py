@@ -208,3 +208,63 @@ def test_modules_compile_with_and_without_gradients(which):
         assert all(torch.equal(u, v) for u, v in zip(ga, gb))
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(outs(c), outs(m)))
+
+
+@pytest.mark.parametrize("M,D", [(5, 96), (700, 1001), (300, 3584), (3, 40000)])
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("e4m3", [True, False])
+def test_stream_written_over_either_of_its_terms(M, D, dt, e4m3):
+    """The C entry points take s = x or s = residual: the same bits."""
+    g = torch.Generator().manual_seed(D)
+    x, r = (torch.randn(M, D, generator=g).to(dt).to(DEV) for _ in range(2))
+    w = torch.ones(D, device=DEV, dtype=dt)
+    code = _lib.F32 if dt == F32 else _lib.BF16
+    eps = ctypes.byref(ctypes.c_float(1e-6))
+    st = torch.cuda.current_stream().cuda_stream
+
+    def run(over):
+        a, b = x.clone(), r.clone()
+        s = {"none": torch.empty_like(x), "x": a, "residual": b}[over]
+        y = torch.empty(M, D, device=DEV, dtype=torch.uint8 if e4m3 else dt)
+        scale, rstd = torch.zeros(M, device=DEV), torch.empty(M, device=DEV)
+        p = [t.data_ptr() for t in (a, b, w, y)] + ([scale.data_ptr()] if e4m3 else []) + [s.data_ptr(), rstd.data_ptr()]
+        _lib.call("swiglu_b200_rmsnorm_fwd_e4m3" if e4m3 else "swiglu_b200_rmsnorm_fwd", *p, M, D, eps, code, code, st)
+        torch.cuda.synchronize()
+        return y, s, rstd, scale
+
+    want = run("none")
+    for over in ("x", "residual"):
+        assert all(torch.equal(a, b) for a, b in zip(run(over), want)), over
+
+
+@pytest.mark.parametrize("M,D", [(3, 128), (640, 1024), (6000, 2048)])
+def test_a_chain_without_a_pause_gives_the_bits_of_one_with_pauses(M, D):
+    """Each kernel is placed while the previous one drains: a chain in which each
+    reads, or writes over, what the one before it wrote or read."""
+    g = torch.Generator().manual_seed(M)
+    x0, r0 = (torch.randn(M, D, generator=g).to(BF).to(DEV) for _ in range(2))
+    w = torch.ones(D, device=DEV, dtype=BF)
+    weight = ops.quantize_mxfp4((torch.randn(D, D, generator=g) * D ** -0.5).to(BF).to(DEV))
+
+    def chain(pause):
+        x, r, norms = x0.clone(), r0.clone(), []
+        wait = torch.cuda.synchronize if pause else lambda: None
+        for _ in range(12):
+            y, s, rstd = ops.rmsnorm_fwd(x, w, r)
+            wait()
+            q = ops.quantize_mxfp4(y)
+            wait()
+            c = ops.matmul_mxfp4(*q, *weight)
+            wait()
+            dx, dw = ops.rmsnorm_bwd(c, s, w, rstd, x)
+            wait()
+            norms.append(ops.clip_grad_norm_([dx, dw], 30.0))      # in place
+            wait()
+            norms.append(ops.clip_grad_norm_([dx, s], 40.0, out=[r, x]))  # over what the norm reads next
+            wait()
+        return x, r, *norms
+
+    want = chain(True)
+    for _ in range(8):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
+    assert ops.device_status(0) == 0
